@@ -4,7 +4,7 @@ ARCH  ?= gfx950
 CSRC  := merv_amd/csrc
 LIB   := merv_amd/lib/libmerv_hip.so
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Wall -Wno-unused-function -Iinclude
-HIP_SRCS := $(CSRC)/gemm.hip $(CSRC)/attention.hip $(CSRC)/rowops.hip $(CSRC)/preproc.hip $(CSRC)/backward.hip $(CSRC)/mxfp8.hip $(CSRC)/decode.hip $(CSRC)/capi.hip
+HIP_SRCS := $(CSRC)/gemm.hip $(CSRC)/attention.hip $(CSRC)/rowops.hip $(CSRC)/preproc.hip $(CSRC)/backward.hip $(CSRC)/mxfp8.hip $(CSRC)/decode.hip $(CSRC)/paged.hip $(CSRC)/capi.hip
 HIP_OBJS := $(HIP_SRCS:.hip=.o)
 
 HOOKS_LIB := merv_amd/lib/libmerv_hip_hooks.so
@@ -17,6 +17,9 @@ lib: $(LIB)
 
 $(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/kernels.h $(CSRC)/prof.h include/merv_hip.h
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
+
+# no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then
+$(CSRC)/paged.o $(HOOKS_DIR)/paged.o: HIPFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 
 $(CSRC)/sampler.o: $(CSRC)/sampler.cpp include/merv_hip.h
 	g++ -O2 -std=c++17 -fPIC -ffp-contract=off -Wall -c $< -o $@

@@ -452,6 +452,56 @@ int merv_decode_sample_advance(const float *logits, int32_t V, const void *param
 int merv_map_pool_attention(const void *kv, const float *q, void *out, int32_t nseq, int32_t ntok, int32_t heads, float scale,
                             void *stream);
 
+/*
+ * A paged key / value cache for batches of rows (sequences) of unlike length, and the attention of one new token for each row over it. The
+ * reference decodes through HF's DynamicCache, one clip a call (merv/models/vidlms/merv.py:818-825); these carry the decoding step of several clips
+ * or questions at once (merv_amd/llm.py, PagedDecoder). They came after ABI version 4's other entries and change none of them.
+ *
+ *  Pages: k_pages / v_pages hold element (page, kv head, slot, d) at page * stride_page + head * stride_head + slot * stride_token + d (the same strides
+ *  for both), bf16 or OCP e4m3. With e4m3, scale byte (page, head, slot) is at page * scale_stride_page + head * scale_stride_head + slot and a number
+ *  stands for code * 2^(byte - 127). table[row * table_stride + i] is the page that holds positions i * page_size .. of a row; entries no call reaches
+ *  may hold anything. Device-side integers are never trusted with an address: see each call for what a bad one does.
+ *  Limits: head_dim 64 or 128; page_size a power of two from 16 to 1024; page and row pointers 16-byte aligned with strides that are multiples of 8 (bf16) or 16
+ *  (e4m3) elements, scale pointers 4-byte aligned with strides that are multiples of 4.
+ */
+enum { MERV_KV_BF16 = 0, MERV_KV_E4M3 = 1 };
+typedef struct merv_paged_cache {
+    void *k_pages, *v_pages;
+    void *k_scales, *v_scales;    /* e4m3 only, else NULL */
+    const int32_t *table;         /* device [rows, table_width] */
+    int64_t n_pages;
+    int64_t stride_page, stride_head, stride_token;      /* in elements */
+    int64_t scale_stride_page, scale_stride_head;
+    int64_t table_stride;
+    int32_t rows, table_width, kv_heads, head_dim, page_size, format;
+} merv_paged_cache;
+/* New tokens into the cache: apply_rotary_pos_emb on k (and q), then the store; v as it is. Token t (0 <= t < T) is row b's where
+ * offsets[b] <= t < offsets[b + 1] (device int32 [rows + 1], not decreasing), at position start[b] + t - offsets[b]; offsets = NULL: one token
+ * a row, T = rows. A row with start[b] < 0 and tokens at or behind offsets[rows] are left alone in every output. k, v [T, kv_heads, hd], q, q_out
+ * [T, heads, hd], k_out [T, kv_heads, hd] bf16 with token and head strides in elements; q = NULL (heads = 0) and k_out = NULL leave these out; q_out may be q
+ * and k_out may be k. cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
+ * rounded to bf16 once. e4m3: a row's scale is the smallest power of two under which no finite element of the (bf16) row is over 448, 2^-126 at least;
+ * the codes are rounded to nearest even; NaN and infinities become NaN. A position without a page in the table is not stored; with rotation, one
+ * outside the tables or without a page is NaN in q_out and k_out. Two tokens of one call must not meet in one slot of one page. */
+int merv_paged_cache_write(const merv_paged_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v, int64_t v_stride,
+                           int64_t v_head_stride, const void *q, int64_t q_stride, int64_t q_head_stride, const void *cos_t, const void *sin_t,
+                           int64_t rope_len, int64_t rope_stride, void *q_out, int64_t q_out_stride, int64_t q_out_head_stride, void *k_out,
+                           int64_t k_out_stride, int64_t k_out_head_stride, const int32_t *offsets, const int32_t *start, int32_t T, int32_t heads,
+                           void *stream);
+/* Cached keys and values back as bf16: k_out, v_out [T, kv_heads, hd]; token t is row b's (offsets as above, required) at position
+ * (start ? start[b] : 0) + t - offsets[b]. A position without a page reads as NaN; rows with start[b] < 0 and tokens behind the last row are left alone. */
+int merv_paged_cache_read(const merv_paged_cache *cache, void *k_out, int64_t k_out_stride, int64_t k_out_head_stride, void *v_out, int64_t v_out_stride,
+                          int64_t v_out_head_stride, const int32_t *offsets, const int32_t *start, int32_t T, void *stream);
+/* out[b, h] = sum_j softmax_j(scale * q[b, h] . k[b, j]) v[b, j] over positions max(0, len - window) .. len - 1 of row b, len = lens[b] (device int32;
+ * window <= 0: all); kv head = h / (heads / kv_heads). lse (may be NULL) [rows, heads] fp32 = ln sum_j exp(scale * q . k). len <= 0: out = 0 and lse = -inf. A
+ * length over the table's capacity or a bad page among those the row reads: that row's out and lse are NaN. Keys and values behind a row's length,
+ * in its last page or before its window, may hold anything, NaN among it. q, out [rows, heads, hd] bf16 by strides; workspace:
+ * merv_paged_decode_attention_workspace_bytes(...) bytes, 16-byte aligned, of any contents, not shared by calls that may run at the same time. */
+size_t merv_paged_decode_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t capacity);
+int merv_paged_decode_attention(const merv_paged_cache *cache, const void *q, int64_t q_stride, int64_t q_head_stride, void *out, int64_t out_stride,
+                                int64_t out_head_stride, float *lse, const int32_t *lens, int32_t heads, int64_t window, float scale, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

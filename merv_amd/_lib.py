@@ -31,6 +31,7 @@ def tuning(name: str, default=None):
     return os.environ.get(name, default) if tuning_hooks_enabled() else default
 
 
+KV_BF16, KV_E4M3 = 0, 1
 ACT = {"none": 0, "gelu_erf": 1, "gelu_tanh": 2, "quick_gelu": 3}
 PIX_LAYOUT = {"BFCHW": 0, "BCFHW": 1}
 DT_F32, DT_BF16 = 0, 1
@@ -61,6 +62,17 @@ class EncoderWeights(C.Structure):
         ("patch_w", C.c_void_p), ("patch_b", C.c_void_p), ("prefix", C.c_void_p), ("pos", C.c_void_p),
         ("pre_ln_w", C.c_void_p), ("pre_ln_b", C.c_void_p), ("final_ln_w", C.c_void_p), ("final_ln_b", C.c_void_p),
         ("layers", C.POINTER(LayerWeights)),
+    ]
+
+
+class PagedCache(C.Structure):
+    """merv_paged_cache: the pages, scales and page table of one call (include/merv_hip.h)."""
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("table", C.c_void_p),
+        ("n_pages", C.c_int64), ("stride_page", C.c_int64), ("stride_head", C.c_int64), ("stride_token", C.c_int64),
+        ("scale_stride_page", C.c_int64), ("scale_stride_head", C.c_int64), ("table_stride", C.c_int64),
+        ("rows", C.c_int32), ("table_width", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+        ("format", C.c_int32),
     ]
 
 
@@ -135,6 +147,11 @@ SIGNATURES = {
     "merv_decode_oproj_merge": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "merv_decode_greedy_advance": (C.c_int, [_vp, _i32, _vp, _vp, _vp, C.c_int64, _vp]),
     "merv_decode_sample_advance": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, C.c_int64, _vp]),
+    "merv_paged_cache_write": (C.c_int, [C.POINTER(PagedCache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                                         _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _vp]),
+    "merv_paged_cache_read": (C.c_int, [C.POINTER(PagedCache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp]),
+    "merv_paged_decode_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64]),
+    "merv_paged_decode_attention": (C.c_int, [C.POINTER(PagedCache), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _f32, _vp, _sz, _vp]),
     "merv_tuning_hooks": (C.c_int, []),
     "merv_debug_set_gemm_variant": (None, [_i32]),
     "merv_debug_set_attn_rescale_thr": (None, [_f32]),

@@ -1141,3 +1141,109 @@ extern "C" int merv_map_pool_attention(const void* kv, const float* q, void* out
     MERV_HIP(launch_map_pool(a, (hipStream_t)stream_));
     return 0;
 }
+
+// ---- paged key / value cache ----
+// The host checks everything that it can see; what lies in device memory (offsets, lengths, table) the kernels check before they use it as an index.
+static bool paged_rows_ok(const void* p, int64_t stride, int64_t head_stride) {
+    return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && head_stride % 8 == 0;
+}
+
+static int paged_cache_args(const merv_paged_cache* c, PagedCacheArgs* a) {
+    MERV_CHECK(c, "paged cache: null argument");
+    MERV_CHECK(c->format == MERV_KV_BF16 || c->format == MERV_KV_E4M3, "paged cache: unknown format");
+    MERV_CHECK(c->rows >= 0 && c->table_width >= 0 && c->n_pages >= 0 && c->kv_heads > 0, "paged cache: bad geometry");
+    MERV_CHECK(c->head_dim == 64 || c->head_dim == 128, "paged cache: head_dim must be 64 or 128");
+    int lg = 4;
+    while (lg < 10 && (1 << lg) != c->page_size) ++lg;
+    MERV_CHECK((1 << lg) == c->page_size, "paged cache: page_size must be a power of two from 16 to 1024");
+    const bool e4m3 = c->format == MERV_KV_E4M3;
+    MERV_CHECK((c->k_pages && c->v_pages) || c->n_pages == 0, "paged cache: null pages");
+    MERV_CHECK(c->table || c->rows == 0 || c->table_width == 0, "paged cache: null table");
+    const int64_t unit = e4m3 ? 16 : 8;
+    MERV_CHECK((((uintptr_t)c->k_pages | (uintptr_t)c->v_pages) & 15) == 0 && c->stride_page % unit == 0 && c->stride_head % unit == 0 &&
+                   c->stride_token % unit == 0,
+               "paged cache: pages must be 16-byte aligned with strides of whole 16-byte units");
+    MERV_CHECK(!e4m3 || (c->k_scales && c->v_scales) || c->n_pages == 0, "paged cache: e4m3 pages need scales");
+    MERV_CHECK(!e4m3 || ((((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 3) == 0 && c->scale_stride_page % 4 == 0 && c->scale_stride_head % 4 == 0),
+               "paged cache: scales must be 4-byte aligned with strides that are multiples of 4");
+    *a = PagedCacheArgs{c->k_pages, c->v_pages, (uint8_t*)c->k_scales, (uint8_t*)c->v_scales, c->table, (long)c->n_pages, (long)c->stride_page,
+                        (long)c->stride_head, (long)c->stride_token, (long)c->scale_stride_page, (long)c->scale_stride_head, (long)c->table_stride,
+                        c->rows, c->table_width, c->kv_heads, c->head_dim, lg, e4m3};
+    return 0;
+}
+
+extern "C" int merv_paged_cache_write(const merv_paged_cache* cache, const void* k, int64_t k_stride, int64_t k_head_stride, const void* v,
+                                      int64_t v_stride, int64_t v_head_stride, const void* q, int64_t q_stride, int64_t q_head_stride,
+                                      const void* cos_t, const void* sin_t, int64_t rope_len, int64_t rope_stride, void* q_out, int64_t q_out_stride,
+                                      int64_t q_out_head_stride, void* k_out, int64_t k_out_stride, int64_t k_out_head_stride,
+                                      const int32_t* offsets, const int32_t* start, int32_t T, int32_t heads, void* stream_) {
+    PagedWriteArgs a{};
+    if (int rc = paged_cache_args(cache, &a.c)) return rc;
+    MERV_CHECK(T >= 0 && heads >= 0, "merv_paged_cache_write: bad geometry");
+    MERV_CHECK(offsets || T == cache->rows, "merv_paged_cache_write: without offsets there is one token for each row");
+    if (T == 0) return 0;
+    MERV_CHECK(k && v && start, "merv_paged_cache_write: null argument");
+    MERV_CHECK((cos_t != nullptr) == (sin_t != nullptr), "merv_paged_cache_write: cos and sin come together");
+    MERV_CHECK((q != nullptr) == (q_out != nullptr) && (!q || (cos_t && heads > 0)), "merv_paged_cache_write: q needs q_out, heads and the rotary tables");
+    MERV_CHECK(!cos_t || (rope_len > 0 && rope_stride >= cache->head_dim && paged_rows_ok(cos_t, rope_stride, 0) && paged_rows_ok(sin_t, rope_stride, 0)),
+               "merv_paged_cache_write: the rotary tables need rows, 16-byte aligned");
+    MERV_CHECK(paged_rows_ok(k, k_stride, k_head_stride) && paged_rows_ok(v, v_stride, v_head_stride) && paged_rows_ok(q, q_stride, q_head_stride) &&
+                   paged_rows_ok(q_out, q_out_stride, q_out_head_stride) && paged_rows_ok(k_out, k_out_stride, k_out_head_stride),
+               "merv_paged_cache_write: rows must be 16-byte aligned with strides that are multiples of 8");
+    a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.q = (const bf16_t*)q;
+    a.cos = (const bf16_t*)cos_t; a.sin = (const bf16_t*)sin_t;
+    a.q_out = (bf16_t*)q_out; a.k_out = (bf16_t*)k_out;
+    a.offsets = offsets; a.start = start;
+    a.k_st = k_stride; a.k_sh = k_head_stride; a.v_st = v_stride; a.v_sh = v_head_stride; a.q_st = q_stride; a.q_sh = q_head_stride;
+    a.qo_st = q_out_stride; a.qo_sh = q_out_head_stride; a.ko_st = k_out_stride; a.ko_sh = k_out_head_stride;
+    a.rope_st = rope_stride; a.rope_len = rope_len;
+    a.T = T; a.H = q ? heads : 0;
+    MERV_STREAM_DEVICE(stream_);
+    MERV_HIP(launch_paged_write(a, (hipStream_t)stream_));
+    return 0;
+}
+
+extern "C" int merv_paged_cache_read(const merv_paged_cache* cache, void* k_out, int64_t k_out_stride, int64_t k_out_head_stride, void* v_out,
+                                     int64_t v_out_stride, int64_t v_out_head_stride, const int32_t* offsets, const int32_t* start, int32_t T,
+                                     void* stream_) {
+    PagedReadArgs a{};
+    if (int rc = paged_cache_args(cache, &a.c)) return rc;
+    MERV_CHECK(T >= 0, "merv_paged_cache_read: bad geometry");
+    if (T == 0) return 0;
+    MERV_CHECK(k_out && v_out && offsets, "merv_paged_cache_read: null argument");
+    MERV_CHECK(paged_rows_ok(k_out, k_out_stride, k_out_head_stride) && paged_rows_ok(v_out, v_out_stride, v_out_head_stride),
+               "merv_paged_cache_read: rows must be 16-byte aligned with strides that are multiples of 8");
+    a.k_out = (bf16_t*)k_out; a.v_out = (bf16_t*)v_out;
+    a.offsets = offsets; a.start = start;
+    a.ko_st = k_out_stride; a.ko_sh = k_out_head_stride; a.vo_st = v_out_stride; a.vo_sh = v_out_head_stride;
+    a.T = T;
+    MERV_STREAM_DEVICE(stream_);
+    MERV_HIP(launch_paged_read(a, (hipStream_t)stream_));
+    return 0;
+}
+
+extern "C" size_t merv_paged_decode_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t capacity) {
+    if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || capacity < 0) return 0;
+    return paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, (long)capacity);
+}
+
+extern "C" int merv_paged_decode_attention(const merv_paged_cache* cache, const void* q, int64_t q_stride, int64_t q_head_stride, void* out,
+                                           int64_t out_stride, int64_t out_head_stride, float* lse, const int32_t* lens, int32_t heads,
+                                           int64_t window, float scale, void* workspace, size_t workspace_bytes, void* stream_) {
+    PagedAttnArgs a{};
+    if (int rc = paged_cache_args(cache, &a.c)) return rc;
+    MERV_CHECK(heads > 0 && heads % cache->kv_heads == 0, "merv_paged_decode_attention: heads must be a multiple of kv_heads");
+    if (cache->rows == 0) return 0;
+    MERV_CHECK(q && out && lens, "merv_paged_decode_attention: null argument");
+    MERV_CHECK(paged_rows_ok(q, q_stride, q_head_stride) && paged_rows_ok(out, out_stride, out_head_stride),
+               "merv_paged_decode_attention: rows must be 16-byte aligned with strides that are multiples of 8");
+    const size_t need = paged_attention_workspace_bytes(cache->rows, heads, cache->kv_heads, cache->head_dim, (long)cache->table_width * cache->page_size);
+    MERV_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+               "merv_paged_decode_attention: workspace too small (merv_paged_decode_attention_workspace_bytes) or not 16-byte aligned");
+    a.q = (const bf16_t*)q; a.out = (bf16_t*)out; a.lse = lse; a.ws = workspace; a.lens = lens;
+    a.q_st = q_stride; a.q_sh = q_head_stride; a.o_st = out_stride; a.o_sh = out_head_stride;
+    a.window = window; a.H = heads; a.scale = scale;
+    MERV_STREAM_DEVICE(stream_);
+    MERV_HIP(launch_paged_attention(a, (hipStream_t)stream_));
+    return 0;
+}

@@ -435,4 +435,46 @@ hipError_t launch_decode_oproj_merge(const DecodeOprojMergeArgs& a, hipStream_t 
 hipError_t launch_decode_greedy_advance(const float* logits, int V, long* tok, long* pos, long* out_tokens, long pos0, hipStream_t s);
 hipError_t launch_decode_sample_advance(const float* logits, int V, const void* params, long* tok, long* pos, long* out_tokens, long pos0, hipStream_t s);
 
+// ---- paged key / value cache (paged.hip) ----
+struct PagedCacheArgs {  // pages [n_pages, kv_heads, 1 << page_log2, hd] by strides (hd contiguous), bf16 or e4m3; k and v share their strides
+    void* k;
+    void* v;
+    uint8_t* k_scale;  // e4m3: one E8M0 byte for each token and head, tokens contiguous
+    uint8_t* v_scale;
+    const int* table;  // [rows, table_width] page numbers
+    long n_pages, s_page, s_head, s_tok, ss_page, ss_head, table_stride;
+    int rows, table_width, kv_heads, hd, page_log2, e4m3;
+};
+struct PagedWriteArgs {
+    PagedCacheArgs c;
+    const bf16_t *k, *v, *q;      // [T, heads, hd] by strides; q may be null
+    const bf16_t *cos, *sin;      // [rope_len, hd], or null: nothing is rotated
+    bf16_t *q_out, *k_out;        // rotated (k_out may be null)
+    const int *offsets, *start;   // offsets [rows + 1] (null: token t is row t's), start [rows]
+    long k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh, ko_st, ko_sh, rope_st, rope_len;
+    int T, H;
+};
+hipError_t launch_paged_write(const PagedWriteArgs& a, hipStream_t s);
+struct PagedReadArgs {
+    PagedCacheArgs c;
+    bf16_t *k_out, *v_out;        // [T, kv_heads, hd] by strides
+    const int *offsets, *start;   // start may be null: 0
+    long ko_st, ko_sh, vo_st, vo_sh;
+    int T;
+};
+hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s);
+struct PagedAttnArgs {
+    PagedCacheArgs c;
+    const bf16_t* q;   // [rows, H, hd] by strides
+    bf16_t* out;
+    float* lse;        // [rows, H] or null
+    void* ws;
+    const int* lens;   // [rows]
+    long q_st, q_sh, o_st, o_sh, window;  // window <= 0: all positions
+    int H;
+    float scale;
+};
+hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
+size_t paged_attention_workspace_bytes(int rows, int H, int kv_heads, int hd, long capacity);
+
 }  // namespace merv

@@ -1,7 +1,7 @@
 """
 Tensor-level wrappers of the single-kernel C-ABI entry points (include/merv_hip.h, "single kernels" section).
 Used by the parity tests and micro-benchmarks; the encoders themselves run through merv_encoder_forward.
-All tensors must be contiguous CUDA (ROCm) tensors: bf16 activations / GEMM weights, fp32 vectors.
+All tensors must be contiguous CUDA (ROCm) tensors: bf16 activations / GEMM weights, fp32 vectors (the paged cache takes strides).
 """
 from __future__ import annotations
 
@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import ACT, DT_BF16, DT_F32, check, current_stream_ptr, ptr
+from ._lib import ACT, DT_BF16, DT_F32, KV_BF16, KV_E4M3, PagedCache, check, current_stream_ptr, ptr
 
 
 def _chk(t: Optional[torch.Tensor], dtype, name: str):
@@ -140,3 +140,160 @@ def gemm_mxfp8(aq, a_sc, wq, w_sc, bias=None, act="none", lscale=None, res=None,
                               aq.stride(0), wq.stride(0), out.stride(0), res.stride(0) if res is not None else 0, ACT[act],
                               current_stream_ptr(aq.device)), "merv_gemm_mxfp8")
     return out
+
+
+# ---- paged key / value cache (PagedDecoder, llm.py): rows of unlike length on one pool of pages ----
+# Pages are [n_pages, kv_heads, page_size, head_dim], bf16 or torch.float8_e4m3fn (then with uint8 scales [n_pages, kv_heads, page_size], a number
+# standing for code * 2^(byte - 127)); table [rows, width] int32 names the page of positions i * page_size .. of a row. Any strides, last
+# dimension contiguous. Row lengths, offsets and page numbers stay on the device (a captured step replays with new ones); the kernels check
+# them: see include/merv_hip.h for what a bad one does. All of this is for inference: no gradients.
+def _stride(t: torch.Tensor, i: int) -> int:
+    return t.stride(i) if t.shape[i] > 1 else 0  # the stride of a dimension of one means nothing
+
+
+def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales) -> PagedCache:
+    if k_pages.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or k_pages.dim() != 4 or not k_pages.is_cuda:
+        raise ValueError(f"{what}: expected CUDA pages [n_pages, kv_heads, page_size, head_dim] of bfloat16 or float8_e4m3fn, got "
+                         f"{k_pages.dtype} {tuple(k_pages.shape)} on {k_pages.device}")
+    n_pages, kv_heads, page, hd = k_pages.shape
+    dev, e4m3 = k_pages.device, k_pages.dtype != torch.bfloat16
+    if v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.device != dev:
+        raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
+    if k_pages.stride(3) != 1:
+        raise ValueError(f"{what}: the pages' last dimension must be contiguous")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: expected an int32 table [rows, width] on {dev} with contiguous rows")
+    ss_page = ss_head = 0
+    if e4m3:
+        if k_scales is None or v_scales is None:
+            raise ValueError(f"{what}: float8_e4m3fn pages need k_scales and v_scales")
+        for s in (k_scales, v_scales):
+            if s.dtype != torch.uint8 or s.shape != k_pages.shape[:3] or s.device != dev or s.stride(2) != 1 or s.stride() != k_scales.stride():
+                raise ValueError(f"{what}: expected uint8 scales {tuple(k_pages.shape[:3])} on {dev}, tokens contiguous, of the same strides")
+        ss_page, ss_head = _stride(k_scales, 0), _stride(k_scales, 1)
+    elif k_scales is not None or v_scales is not None:
+        raise ValueError(f"{what}: bfloat16 pages take no scales")
+    return PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if e4m3 else 0, v_scales.data_ptr() if e4m3 else 0, table.data_ptr(),
+                      n_pages, _stride(k_pages, 0), _stride(k_pages, 1), _stride(k_pages, 2), ss_page, ss_head, _stride(table, 0), table.shape[0],
+                      table.shape[1], kv_heads, hd, page, KV_E4M3 if e4m3 else KV_BF16)
+
+
+def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev, out: bool = False):
+    if t.dtype != torch.bfloat16 or t.shape != shape or t.device != dev or t.stride(2) != 1:
+        raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on {dev} with contiguous last dimension, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    if out and (t.stride(0) == 0 and shape[0] > 1 or t.stride(1) == 0 and shape[1] > 1):
+        raise ValueError(f"{what}: {name}: an output's rows must not share memory")
+    return t.data_ptr(), _stride(t, 0), _stride(t, 1)
+
+
+def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev) -> int:
+    if t is None:
+        return 0
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _launch_on(dev, call, what: str, *args) -> None:
+    """call(*args, stream) on the device's current stream; the device is made current where it is not (its null stream has no device of its own)."""
+    if torch.cuda.current_device() == dev.index:
+        check(call(*args, current_stream_ptr(dev)), what)
+    else:
+        with torch.cuda.device(dev):
+            check(call(*args, current_stream_ptr(dev)), what)
+
+
+def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
+                      offsets: Optional[torch.Tensor] = None, *, k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+                      q: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                      q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """New tokens k, v [T, kv_heads, head_dim] bf16 into the pages, in one launch with the rotary embedding of k and of q [T, heads, head_dim] where
+    cos, sin [positions, head_dim] bf16 are given. Token t is row b's where offsets[b] <= t < offsets[b + 1] (int32 [rows + 1]; None: one token a
+    row, t = b), at position start[b] + t - offsets[b]; rows with start[b] < 0 and tokens behind offsets[rows] are left alone, in every output. Returns
+    the rotated queries (q_out, or a new tensor; q_out=q rotates in place), None without q; k_out takes the rotated keys as well. float8_e4m3fn pages:
+    quantised with one power-of-two scale for each token and head (k_scales, v_scales); what is not finite becomes NaN."""
+    what = "paged_cache_write"
+    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
+    for t in (k_pages, k_scales):
+        if t is not None and any(t.stride(i) == 0 and t.shape[i] > 1 for i in range(3)):
+            raise ValueError(f"{what}: pages and scales must not share memory among themselves")
+    dev = k_pages.device
+    if k.dim() != 3:
+        raise ValueError(f"{what}: k: expected [tokens, kv_heads, head_dim], got {tuple(k.shape)}")
+    T, shape = k.shape[0], (k.shape[0], cache.kv_heads, cache.head_dim)
+    if offsets is None and T != cache.rows:
+        raise ValueError(f"{what}: without offsets there is one token for each row: {T} tokens, {cache.rows} rows")
+    kr, vr = _paged_rows(what, "k", k, shape, dev), _paged_rows(what, "v", v, shape, dev)
+    off_p, start_p = _paged_ints(what, "offsets", offsets, cache.rows + 1, dev), _paged_ints(what, "start", start, cache.rows, dev)
+    if (cos is None) != (sin is None) or (q is not None and cos is None) or (q_out is not None and q is None):
+        raise ValueError(f"{what}: cos and sin come together, q needs them, and q_out needs q")
+    rope = (0, 0, 0, 0)
+    if cos is not None:
+        for t in (cos, sin):
+            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != cache.head_dim or t.device != dev \
+                    or t.stride(1) != 1 or t.stride() != cos.stride():
+                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {cache.head_dim}] on {dev} with contiguous rows, of the same strides")
+        rope = (cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else cos.shape[1])
+    heads, qr, qo = 0, (0, 0, 0), (0, 0, 0)
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != cache.head_dim:
+            raise ValueError(f"{what}: q: expected [{T}, heads, {cache.head_dim}], got {tuple(q.shape)}")
+        heads = q.shape[1]
+        qr = _paged_rows(what, "q", q, q.shape, dev)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        qo = _paged_rows(what, "q_out", q_out, q.shape, dev, True)
+    ko = _paged_rows(what, "k_out", k_out, shape, dev, True) if k_out is not None else (0, 0, 0)
+    _launch_on(dev, _lib.load().merv_paged_cache_write, "merv_paged_cache_write", cache, *kr, *vr, *qr, *rope, *qo, *ko, off_p, start_p, T, heads)
+    return q_out
+
+
+def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, start: Optional[torch.Tensor], offsets: torch.Tensor,
+                     total: int, *, k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None,
+                     k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
+    """Cached keys and values, back as bf16 [total, kv_heads, head_dim] each, rows one behind the other: output t is row b's position
+    (start[b] or 0) + t - offsets[b] where offsets[b] <= t < offsets[b + 1]. Outputs behind offsets[rows], and those of rows with start[b] < 0, are
+    not written. A position without a page reads as NaN. Numbers are given back exactly as the cache holds them."""
+    what = "paged_cache_read"
+    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
+    dev, shape = k_pages.device, (int(total), cache.kv_heads, cache.head_dim)
+    if total < 0 or offsets is None:
+        raise ValueError(f"{what}: total must not be negative, and offsets are needed")
+    off_p, start_p = _paged_ints(what, "offsets", offsets, cache.rows + 1, dev), _paged_ints(what, "start", start, cache.rows, dev)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    ko, vo = _paged_rows(what, "k_out", k_out, shape, dev, True), _paged_rows(what, "v_out", v_out, shape, dev, True)
+    _launch_on(dev, _lib.load().merv_paged_cache_read, "merv_paged_cache_read", cache, *ko, *vo, off_p, start_p, int(total))
+    return k_out, v_out
+
+
+def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
+                           k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                           window: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of one token for each row, q [rows, heads, head_dim] bf16, over positions max(0, lens[b] - window) .. lens[b] - 1 of the row's pages
+    (window 0: all of them; kv head = head // (heads // kv_heads); scale None: head_dim^-0.5). Returns out, or (out, lse [rows, heads] fp32, the
+    natural logarithm of the softmax's sum). A row of length 0 gives zeros and -inf; a length over the table's capacity or a bad page gives
+    that row NaN. Sums, softmax and the weights of the values are held in fp32 (the weights as two bf16 numbers); rounded to bf16 once, at the end."""
+    what = "paged_decode_attention"
+    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
+    dev = k_pages.device
+    if q.dim() != 3 or q.shape[0] != cache.rows or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"{what}: q: expected [{cache.rows}, heads, {cache.head_dim}] with heads a multiple of {cache.kv_heads}, got {tuple(q.shape)}")
+    if window < 0:
+        raise ValueError(f"{what}: window must not be negative")
+    heads = q.shape[1]
+    qr, lens_p = _paged_rows(what, "q", q, q.shape, dev), _paged_ints(what, "lens", lens, cache.rows, dev)
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    orow = _paged_rows(what, "out", out, q.shape, dev, True)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    lib = _lib.load()
+    # a workspace of its own for each call (and each captured graph): nothing is shared by calls that run at the same time
+    nbytes = lib.merv_paged_decode_attention_workspace_bytes(cache.rows, heads, cache.kv_heads, cache.head_dim, cache.table_width * cache.page_size)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch_on(dev, lib.merv_paged_decode_attention, what, cache, *qr, *orow, ptr(lse), lens_p, heads, int(window),
+               cache.head_dim**-0.5 if scale is None else float(scale), ptr(ws), nbytes)
+    return (out, lse) if return_lse else out
