@@ -15,7 +15,7 @@ all: lib hooks oracle
 
 lib: $(LIB)
 
-$(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/kernels.h $(CSRC)/prof.h include/merv_hip.h
+$(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/kernels.h $(CSRC)/paged_split.h $(CSRC)/prof.h include/merv_hip.h
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then
@@ -35,7 +35,7 @@ $(LIB): $(HIP_OBJS) $(CSRC)/sampler.o $(CSRC)/prof.o
 # test / probe infrastructure, loaded only under MERV_TUNING_HOOKS=1 (merv_amd/_lib.py). The product library above has none of it.
 hooks: $(HOOKS_LIB)
 
-$(HOOKS_DIR)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/kernels.h $(CSRC)/prof.h include/merv_hip.h
+$(HOOKS_DIR)/%.o: $(CSRC)/%.hip $(CSRC)/common.h $(CSRC)/kernels.h $(CSRC)/paged_split.h $(CSRC)/prof.h include/merv_hip.h
 	@mkdir -p $(HOOKS_DIR)
 	$(HIPCC) $(HIPFLAGS) -DMERV_TUNING_HOOKS -c $< -o $@
 

@@ -10,6 +10,7 @@
 #include "../../include/merv_hip.h"
 #include "common.h"
 #include "kernels.h"
+#include "paged_split.h"
 
 using namespace merv;
 
@@ -1234,6 +1235,9 @@ extern "C" int merv_paged_decode_attention(const merv_paged_cache* cache, const 
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
     MERV_CHECK(heads > 0 && heads % cache->kv_heads == 0, "merv_paged_decode_attention: heads must be a multiple of kv_heads");
     if (cache->rows == 0) return 0;
+    MERV_CHECK((int64_t)cache->rows * heads < (1LL << 31) && cache->stride_token >= 0 && cache->stride_token < (1LL << 26) &&
+                   ((int64_t)cache->table_width * cache->page_size / PAGED_UNIT + 1) * cache->rows < (1LL << 31),
+               "merv_paged_decode_attention: rows * heads and the table's units of 128 positions must fit 31 bits, the token stride 26");
     MERV_CHECK(q && out && lens, "merv_paged_decode_attention: null argument");
     MERV_CHECK(paged_rows_ok(q, q_stride, q_head_stride) && paged_rows_ok(out, out_stride, out_head_stride),
                "merv_paged_decode_attention: rows must be 16-byte aligned with strides that are multiples of 8");

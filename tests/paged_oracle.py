@@ -36,8 +36,8 @@ def attention(q, k_rows, v_rows, scale, window=0):
     """q [rows, H, hd]; k_rows, v_rows: lists of [len, Hkv, hd]. -> out, lse (float64) and how far a result in fp32 that is rounded to bf16 may be off each.
 
     With p the softmax, s the scores and u = 2^-24: a score is a sum of hd products, exact in fp32, off by at most (hd + 3) u scale sum |q k| =: d
-    (the 3: the factors scale, log2 e and their product), and exp2's argument and result add (|s| + 2) 2^-22; a weight is two bf16 numbers, off by
-    2^-16; numerator and denominator are sums of len terms, (len + 8) u each (8: joining the parts of a split). out is a quotient, so each counts
+    (the 3: the factors scale, log2 e and their product), and exp2's argument and result add (|s| + 2) 2^-22; a weight is two bf16
+    numbers: cut off after 8 bits, a rest under 2^-7 of it, which is rounded to 8 bits: off by 2^-8 2^-7 = 2^-15; numerator and denominator are sums of len terms, (len + 8) u each (8: joining the parts of a split). out is a quotient, so each counts
     twice, times sum p |v|; then 2^-8 |out| for the rounding to bf16."""
     rows, H, hd = q.shape
     out, lse = torch.zeros(rows, H, hd, dtype=F64), torch.full((rows, H), -math.inf, dtype=F64)
@@ -56,7 +56,7 @@ def attention(q, k_rows, v_rows, scale, window=0):
             p = torch.softmax(s, -1)
             out[b, h], lse[b, h] = p @ v[:, g], torch.logsumexp(s, -1)
             d = (hd + 3) * u * scale * float((k[:, g].abs() @ x.abs()).max()) + (float(s.abs().max()) + 2) * 2.0**-22
-            one = d + 2.0**-16 + (n + 8) * u
+            one = d + 2.0**-15 + (n + 8) * u
             out_tol[b, h] = 2 * one * (p @ v[:, g].abs()) + 2.0**-8 * out[b, h].abs() + 1e-30
             lse_tol[b, h] = d + (n + 8) * u + float(lse[b, h].abs() + 1) * 2.0**-22
     return out, lse, out_tol, lse_tol

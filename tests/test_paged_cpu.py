@@ -75,3 +75,88 @@ def test_tensors_on_the_cpu_are_refused():
         ops.paged_cache_read(pages, pages, table, None, torch.zeros(4, dtype=torch.int32), 0)
     with pytest.raises(ValueError, match="CUDA"):
         ops.paged_decode_attention(q, pages, pages, table, n)
+
+
+PLAN = r"""
+#include <vector>
+#include "paged_split.h"
+using namespace merv;
+// 0: every unit of every row's pairs is done once, by a worker that has it in the segment it is said to, into a slot of its own, and the join
+// of a pair reads just the slots that were written for it; else a number that names what is wrong
+extern "C" int walk(const int* lens, int rows, int pairs, long window, long capacity, int most, int* used) {
+    long total = 0;
+    std::vector<long> first(rows + 1);
+    for (int r = 0; r < rows; ++r) {
+        const PagedSpan s = paged_span(lens[r], window, capacity);
+        if (lens[r] > 0 && lens[r] <= capacity) {
+            if (s.units < 1 || s.base % 16 || s.base > s.lo || s.lo - s.base > 15) return 1;
+            if (s.base + (long)s.units * PAGED_UNIT < s.len || s.base + (long)(s.units - 1) * PAGED_UNIT >= s.len) return 2;
+            if (s.len - s.lo != (window > 0 && window < lens[r] ? window : lens[r])) return 3;
+        } else if (s.units) return 4;
+        first[r] = total;
+        total += (long)s.units * pairs;
+    }
+    first[rows] = total;
+    const int W = paged_workers(total, most);
+    *used = W;
+    std::vector<int> done(total), slot_of(total, -1), taken(2 * (most > 0 ? most : 1));
+    for (int w = 0; w < W; ++w) {
+        const long a = paged_start(w, total, W), b = paged_start(w + 1, total, W);
+        if (b - a < total / W || b - a > total / W + 1 || b <= a) return 5;
+        for (long x = a; x < b;) {
+            if (paged_owner(x, total, W) != w || paged_owner(b - 1, total, W) != w) return 6;
+            int r = 0;
+            while (first[r + 1] <= x) ++r;
+            const int n = paged_span(lens[r], window, capacity).units, u = (int)((x - first[r]) % n);
+            const long m = n - u < b - x ? n - u : b - x;
+            const int slot = m == n ? -1 : x == a ? 2 * w : 2 * w + 1;
+            if (slot >= 0 && taken[slot]++) return 7;
+            for (long y = x; y < x + m; ++y) done[y]++, slot_of[y] = slot;
+            x += m;
+        }
+    }
+    for (long x = 0; x < total; ++x) if (done[x] != 1) return 8;
+    for (int r = 0; r < rows; ++r) {
+        const int n = paged_span(lens[r], window, capacity).units;
+        for (int p = 0; n && p < pairs; ++p) {
+            const long f = first[r] + (long)p * n;
+            const int w0 = paged_owner(f, total, W), w1 = paged_owner(f + n - 1, total, W);
+            if (w0 == w1) { if (slot_of[f] != -1 || slot_of[f + n - 1] != -1) return 9; continue; }
+            for (int w = w0; w <= w1; ++w) {
+                const long at = paged_start(w, total, W) > f ? paged_start(w, total, W) : f;
+                if (at >= f + n || slot_of[at] != paged_slot(w, f, total, W)) return 10;
+            }
+        }
+    }
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def walk(tmp_path_factory):
+    import subprocess
+    from pathlib import Path
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(PLAN)
+    csrc = Path(__file__).resolve().parent.parent / "merv_amd" / "csrc"
+    subprocess.check_call(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", f"-I{csrc}", "-o", str(d / "plan.so"), str(d / "plan.cpp")])
+    fn = C.CDLL(str(d / "plan.so")).walk
+    fn.argtypes = [C.POINTER(C.c_int), C.c_int, C.c_int, C.c_long, C.c_long, C.c_int, C.POINTER(C.c_int)]
+    return fn
+
+
+def test_the_work_is_shared_out_whole(walk):
+    """The split of the one-token attention over workgroups (paged_split.h): any lengths (none, too long, negative), windows, heads, worker counts."""
+    import random
+    rng = random.Random(0)
+    cases = [([1], 1, 0, 64, 512), ([131072], 8, 0, 131072, 512), ([0, 0], 4, 0, 64, 512), ([-5, 3, 10**6], 2, 0, 256, 512), ([129], 1, 1, 256, 512)]
+    for _ in range(400):
+        top = rng.choice([5, 130, 1000, 6000])
+        cases.append(([rng.randint(-1, top + 3) for _ in range(rng.randint(1, 40))], rng.randint(1, 9), rng.choice([0, 0, 1, 15, 16, 17, rng.randint(1, top)]), top,
+                      rng.choice([1, 2, 3, 7, 64, 512])))
+    for lens, pairs, window, capacity, most in cases:
+        used = C.c_int(-1)
+        rc = walk((C.c_int * len(lens))(*lens), len(lens), pairs, window, capacity, most, C.byref(used))
+        assert rc == 0, (rc, lens, pairs, window, capacity, most)
+        assert 0 <= used.value <= most
