@@ -1180,7 +1180,8 @@ extern "C" int merv_paged_cache_write(const merv_paged_cache* cache, const void*
                                       const int32_t* offsets, const int32_t* start, int32_t T, int32_t heads, void* stream_) {
     PagedWriteArgs a{};
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
-    MERV_CHECK(T >= 0 && heads >= 0, "merv_paged_cache_write: bad geometry");
+    MERV_CHECK(T >= 0 && heads >= 0 && heads <= 65536 && cache->kv_heads <= 65536 && (int64_t)T * (2 * (int64_t)cache->kv_heads + heads) < (1LL << 36),
+               "merv_paged_cache_write: bad geometry");
     MERV_CHECK(offsets || T == cache->rows, "merv_paged_cache_write: without offsets there is one token for each row");
     if (T == 0) return 0;
     MERV_CHECK(k && v && start, "merv_paged_cache_write: null argument");
@@ -1209,7 +1210,7 @@ extern "C" int merv_paged_cache_read(const merv_paged_cache* cache, void* k_out,
                                      void* stream_) {
     PagedReadArgs a{};
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
-    MERV_CHECK(T >= 0, "merv_paged_cache_read: bad geometry");
+    MERV_CHECK(T >= 0 && cache->kv_heads <= 65536 && (int64_t)T * cache->kv_heads < (1LL << 35), "merv_paged_cache_read: bad geometry");
     if (T == 0) return 0;
     MERV_CHECK(k_out && v_out && offsets, "merv_paged_cache_read: null argument");
     MERV_CHECK(paged_rows_ok(k_out, k_out_stride, k_out_head_stride) && paged_rows_ok(v_out, v_out_stride, v_out_head_stride),
@@ -1235,18 +1236,19 @@ extern "C" int merv_paged_decode_attention(const merv_paged_cache* cache, const 
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
     MERV_CHECK(heads > 0 && heads % cache->kv_heads == 0, "merv_paged_decode_attention: heads must be a multiple of kv_heads");
     if (cache->rows == 0) return 0;
-    MERV_CHECK((int64_t)cache->rows * heads < (1LL << 31) && cache->stride_token >= 0 && cache->stride_token < (1LL << 26) &&
-                   ((int64_t)cache->table_width * cache->page_size / PAGED_UNIT + 1) * cache->rows < (1LL << 31),
-               "merv_paged_decode_attention: rows * heads and the table's units of 128 positions must fit 31 bits, the token stride 26");
+    const int64_t capacity = (int64_t)cache->table_width * cache->page_size;
+    MERV_CHECK(capacity <= (1LL << 30) && cache->stride_token >= 0 && cache->stride_token < (1LL << 26) &&
+                   (capacity / PAGED_UNIT + 1) * cache->rows * heads < (1LL << 31),
+               "merv_paged_decode_attention: at most 2^30 positions a row, 2^31 units of 128 positions over all rows and heads, a token stride under 2^26");
     MERV_CHECK(q && out && lens, "merv_paged_decode_attention: null argument");
     MERV_CHECK(paged_rows_ok(q, q_stride, q_head_stride) && paged_rows_ok(out, out_stride, out_head_stride),
                "merv_paged_decode_attention: rows must be 16-byte aligned with strides that are multiples of 8");
-    const size_t need = paged_attention_workspace_bytes(cache->rows, heads, cache->kv_heads, cache->head_dim, (long)cache->table_width * cache->page_size);
+    const size_t need = paged_attention_workspace_bytes(cache->rows, heads, cache->kv_heads, cache->head_dim, (long)capacity);
     MERV_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "merv_paged_decode_attention: workspace too small (merv_paged_decode_attention_workspace_bytes) or not 16-byte aligned");
     a.q = (const bf16_t*)q; a.out = (bf16_t*)out; a.lse = lse; a.ws = workspace; a.lens = lens;
     a.q_st = q_stride; a.q_sh = q_head_stride; a.o_st = out_stride; a.o_sh = out_head_stride;
-    a.window = window; a.H = heads; a.scale = scale;
+    a.window = window > 0 && window < capacity ? (int)window : 0; a.H = heads; a.scale = scale;
     MERV_STREAM_DEVICE(stream_);
     MERV_HIP(launch_paged_attention(a, (hipStream_t)stream_));
     return 0;

@@ -470,8 +470,8 @@ struct PagedAttnArgs {
     float* lse;        // [rows, H] or null
     void* ws;
     const int* lens;   // [rows]
-    long q_st, q_sh, o_st, o_sh, window;  // window <= 0: all positions
-    int H;
+    long q_st, q_sh, o_st, o_sh;
+    int H, window;     // window 0: all positions
     float scale;
     int head_blocks, workers;  // set by the launch
 };

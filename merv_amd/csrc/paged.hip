@@ -21,9 +21,9 @@ MERV_DEVICE void unpack8f(const u32x4 r, float* f) {
     }
 }
 
-// the row a new token belongs to: how many of offsets[1 .. rows] are <= t, 64 at a time (independent loads, one round trip for up to 64 rows, where a
+// the row a token belongs to: how many of offsets[1 .. rows] are <= t, 64 at a time (independent loads, one round trip for up to 64 rows, where a
 // binary search would make six dependent ones). rows: behind the last row. Called by whole waves with a uniform t.
-MERV_DEVICE int row_of_token(const int* offsets, int rows, int t) {
+MERV_DEVICE int row_of_token(const int* offsets, int rows, long t) {
     const int lane = threadIdx.x & 63;
     int n = 0;
     for (int base = 1; base <= rows; base += 64) {
@@ -33,20 +33,32 @@ MERV_DEVICE int row_of_token(const int* offsets, int rows, int t) {
     return n;
 }
 
+// the same for any lane's t, from a row at or before it: mostly that row or, a few steps on, the next one that has tokens
+MERV_DEVICE int row_from(const int* offsets, int rows, int row, long t) {
+    if (row >= rows || offsets[row + 1] > t) return row;
+    int lo = row + 1, hi = rows;  // the first row in [lo, hi) whose end is behind t, or rows
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (offsets[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
 struct TokenPlace {
     long pos;   // the token's position in its row
     long page;  // its page's number, -1: it has none
     bool idle;  // belongs to no row, or to one that sits this call out
 };
 
-MERV_DEVICE TokenPlace place_of_token(const PagedCacheArgs& c, const int* offsets, const int* start, int t) {
+MERV_DEVICE TokenPlace place_of_token(const PagedCacheArgs& c, const int* offsets, const int* start, long t, int row) {
     TokenPlace p{0, -1, true};
-    const int row = offsets ? row_of_token(offsets, c.rows, t) : t;
     if (row >= c.rows) return p;
-    const int first = offsets ? offsets[row] : t, s = start ? start[row] : 0;
+    const long first = offsets ? offsets[row] : t;
+    const int s = start ? start[row] : 0;
     if (s < 0 || t < first) return p;
     p.idle = false;
-    p.pos = (long)s + (t - first);
+    p.pos = s + (t - first);
     const long col = p.pos >> c.page_log2;
     if (col < c.table_width) {
         const int id = c.table[(long)row * c.table_stride + col];
@@ -91,32 +103,49 @@ MERV_DEVICE void e4m3_unpack8(const u32x2 r, float* f) {
 }
 
 // ---- write ----
-// One block per new token. A lane holds elements d .. d + 7 of one head's vector and their partners d + hd/2 .. (the rotation mixes just these), so
-// hd / 16 lanes hold a vector and the queries may be rotated in place. rot(x) = x cos + rotate_half(x) sin: with bf16 operands and bf16 tables both
-// products are exact in fp32, so the sum's rounding to fp32 and its rounding to bf16 are the only two.
-template <int HD, bool E4M3>
+// All vectors of the call (a token's keys, values and queries, token after token) are one line; a block takes WRITE_EACH x 256 / (hd / 16) of them, so it is full
+// whatever the numbers of heads are. A lane holds elements d .. d + 7 of a vector and their partners d + hd/2 .. (the rotation mixes just these), so
+// hd / 16 lanes hold a vector and queries and keys may be rotated in place. The vectors are requested before their places are looked up: the two chains of loads
+// overlap. rot(x) = x cos + rotate_half(x) sin: with bf16 operands and bf16 tables both products are exact in fp32, so the sum's rounding to
+// fp32 and its rounding to bf16 are the only two.
+template <int HD, bool E4M3, int WRITE_EACH>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
     constexpr int LPV = HD / 16, VPB = 256 / LPV;  // lanes for a vector, vectors a block holds at a time
-    const int t = blockIdx.x;
-    const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t);
-    if (at.idle) return;
-    const int sub = threadIdx.x % LPV, d0 = sub * 8;
-    const bool rotate = p.cos != nullptr;
-    const bool in_tables = at.pos < p.rope_len;
-    const int Hkv = p.c.kv_heads, nvec = 2 * Hkv + (p.q ? p.H : 0);
-    const long slot = at.pos & ((1 << p.c.page_log2) - 1);
-    for (int i = threadIdx.x / LPV; i < nvec; i += VPB) {
+    const int Hkv = p.c.kv_heads, nvec = 2 * Hkv + p.H;
+    const long v0 = (long)blockIdx.x * (VPB * WRITE_EACH), t0 = v0 / nvec;
+    const int r0 = (int)(v0 - t0 * nvec), sub = threadIdx.x % LPV, d0 = sub * 8;
+    long t[WRITE_EACH];
+    int vec[WRITE_EACH];
+    u32x4 raw[WRITE_EACH][2];
+#pragma unroll
+    for (int e = 0; e < WRITE_EACH; ++e) {
+        const unsigned x = r0 + e * VPB + threadIdx.x / LPV;
+        t[e] = t0 + x / (unsigned)nvec;
+        const int i = vec[e] = x % (unsigned)nvec;
+        const bf16_t* src = i >= 2 * Hkv ? p.q + t[e] * p.q_st + (long)(i - 2 * Hkv) * p.q_sh
+                            : i < Hkv    ? p.k + t[e] * p.k_st + (long)i * p.k_sh
+                                         : p.v + t[e] * p.v_st + (long)(i - Hkv) * p.v_sh;
+        if (t[e] < p.T) {
+            raw[e][0] = *(const u32x4*)(src + d0);
+            raw[e][1] = *(const u32x4*)(src + d0 + HD / 2);
+        }
+    }
+    const int row0 = p.offsets ? row_of_token(p.offsets, p.c.rows, t0) : 0;
+#pragma unroll
+    for (int e = 0; e < WRITE_EACH; ++e) {
+        if (t[e] >= p.T) break;
+        const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t[e], p.offsets ? row_from(p.offsets, p.c.rows, row0, t[e]) : (int)t[e]);
+        if (at.idle) continue;
+        const int i = vec[e];
         const bool is_k = i < Hkv, is_q = i >= 2 * Hkv;
         const int h = is_q ? i - 2 * Hkv : is_k ? i : i - Hkv;
-        const bf16_t* src = is_q ? p.q + (long)t * p.q_st + (long)h * p.q_sh
-                                 : is_k ? p.k + (long)t * p.k_st + (long)h * p.k_sh : p.v + (long)t * p.v_st + (long)h * p.v_sh;
-        float lo[8], hi[8];
-        unpack8f(*(const u32x4*)(src + d0), lo);
-        unpack8f(*(const u32x4*)(src + d0 + HD / 2), hi);
-        u32x4 olo, ohi;
-        if (rotate && (is_k || is_q)) {
-            float cl[8], ch[8], sl[8], sh[8];
-            const bool ok = in_tables && at.page >= 0;
+        const long slot = at.pos & ((1 << p.c.page_log2) - 1);
+        u32x4 olo = raw[e][0], ohi = raw[e][1];
+        if (p.cos && (is_k || is_q)) {
+            float lo[8], hi[8], cl[8], ch[8], sl[8], sh[8];
+            unpack8f(olo, lo);
+            unpack8f(ohi, hi);
+            const bool in_tables = at.pos < p.rope_len, ok = in_tables && at.page >= 0;
             const long row = in_tables ? at.pos : 0;
             unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0), cl);
             unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0 + HD / 2), ch);
@@ -128,19 +157,20 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
                 lo[j] = ok ? a * cl[j] - b * sl[j] : __builtin_nanf("");
                 hi[j] = ok ? b * ch[j] + a * sh[j] : __builtin_nanf("");
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            olo[j] = pack2bf(lo[2 * j], lo[2 * j + 1]);
-            ohi[j] = pack2bf(hi[2 * j], hi[2 * j + 1]);
+            for (int j = 0; j < 4; ++j) {
+                olo[j] = pack2bf(lo[2 * j], lo[2 * j + 1]);
+                ohi[j] = pack2bf(hi[2 * j], hi[2 * j + 1]);
+            }
         }
         if (is_q || (is_k && p.k_out)) {
-            bf16_t* dst = is_q ? p.q_out + (long)t * p.qo_st + (long)h * p.qo_sh : p.k_out + (long)t * p.ko_st + (long)h * p.ko_sh;
+            bf16_t* dst = is_q ? p.q_out + t[e] * p.qo_st + (long)h * p.qo_sh : p.k_out + t[e] * p.ko_st + (long)h * p.ko_sh;
             *(u32x4*)(dst + d0) = olo;
             *(u32x4*)(dst + d0 + HD / 2) = ohi;
         }
         if (is_q) continue;
         if constexpr (E4M3) {
+            float lo[8], hi[8];
             unpack8f(olo, lo);  // the cache's numbers are bf16 ones, whichever way it holds them
             unpack8f(ohi, hi);
             float amax = 0.f;
@@ -148,13 +178,13 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(finite_abs(lo[j]), finite_abs(hi[j])));
 #pragma unroll
             for (int o = LPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-            const int e = row_exponent(amax);
-            const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+            const int ex = row_exponent(amax);
+            const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
             if (at.page < 0) continue;
             uint8_t* dst = (uint8_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
             *(u32x2*)(dst + d0) = u32x2{e4m3_pack4(lo, inv), e4m3_pack4(lo + 4, inv)};
             *(u32x2*)(dst + d0 + HD / 2) = u32x2{e4m3_pack4(hi, inv), e4m3_pack4(hi + 4, inv)};
-            if (sub == 0) (is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] = (uint8_t)(e + 127);
+            if (sub == 0) (is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] = (uint8_t)(ex + 127);
         } else {
             if (at.page < 0) continue;
             bf16_t* dst = (bf16_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
@@ -165,32 +195,54 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
 }
 
 // ---- read ----
-template <int HD, bool E4M3>
+// The same line of vectors, READ_EACH for each group of lanes: all places first, then all loads, then all stores. A lane moves 16 bytes of the cache.
+template <int HD, bool E4M3, int READ_EACH>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
-    constexpr int LPV = HD / 8, VPB = 256 / LPV;
-    const int t = blockIdx.x;
-    const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t);
-    if (at.idle) return;
-    const int d0 = (threadIdx.x % LPV) * 8, Hkv = p.c.kv_heads;
-    const long slot = at.pos & ((1 << p.c.page_log2) - 1);
-    for (int i = threadIdx.x / LPV; i < 2 * Hkv; i += VPB) {
+    constexpr int LPV = E4M3 ? HD / 16 : HD / 8, VPB = 256 / LPV, EPL = HD / LPV;
+    const int Hkv = p.c.kv_heads, nvec = 2 * Hkv;
+    const long v0 = (long)blockIdx.x * (VPB * READ_EACH), t0 = v0 / nvec;
+    const int r0 = (int)(v0 - t0 * nvec), d0 = (threadIdx.x % LPV) * EPL;
+    int row = row_of_token(p.offsets, p.c.rows, t0);
+    bf16_t* dst[READ_EACH];
+    u32x4 x[READ_EACH];
+    int ex[READ_EACH];
+#pragma unroll
+    for (int e = 0; e < READ_EACH; ++e) {
+        const unsigned y = r0 + e * VPB + threadIdx.x / LPV;
+        const long t = t0 + y / (unsigned)nvec;
+        const int i = y % (unsigned)nvec;
+        dst[e] = nullptr;
+        if (t >= p.T) continue;
+        row = row_from(p.offsets, p.c.rows, row, t);
+        const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t, row);
+        if (at.idle) continue;
         const bool is_k = i < Hkv;
         const int h = is_k ? i : i - Hkv;
-        u32x4 o = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};  // NaN: a position without a page
-        if (at.page >= 0) {
-            const long off = at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok + d0;
-            if constexpr (E4M3) {
-                float f[8];
-                e4m3_unpack8(*(const u32x2*)((const uint8_t*)(is_k ? p.c.k : p.c.v) + off), f);
-                const int e = (int)(is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] - 127;
+        const long slot = at.pos & ((1 << p.c.page_log2) - 1);
+        dst[e] = (is_k ? p.k_out + t * p.ko_st + (long)h * p.ko_sh : p.v_out + t * p.vo_st + (long)h * p.vo_sh) + d0;
+        const uint32_t nan = E4M3 ? 0x7f7f7f7fu : 0x7fc07fc0u;  // a position without a page
+        x[e] = u32x4{nan, nan, nan, nan};
+        ex[e] = 0;
+        if (at.page < 0) continue;
+        const long off = at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok + d0;
+        x[e] = *(const u32x4*)((const char*)(is_k ? p.c.k : p.c.v) + off * (E4M3 ? 1 : 2));
+        if constexpr (E4M3) ex[e] = (int)(is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] - 127;
+    }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = pack2bf(ldexpf(f[2 * j], e), ldexpf(f[2 * j + 1], e));
-            } else {
-                o = *(const u32x4*)((const bf16_t*)(is_k ? p.c.k : p.c.v) + off);
-            }
+    for (int e = 0; e < READ_EACH; ++e) {
+        if (!dst[e]) continue;
+        if constexpr (E4M3) {
+            float f[16];
+            e4m3_unpack8(u32x2{x[e][0], x[e][1]}, f);
+            e4m3_unpack8(u32x2{x[e][2], x[e][3]}, f + 8);
+            u32x4 o[2];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j >> 2][j & 3] = pack2bf(ldexpf(f[2 * j], ex[e]), ldexpf(f[2 * j + 1], ex[e]));
+            *(u32x4*)dst[e] = o[0];
+            *(u32x4*)(dst[e] + 8) = o[1];
+        } else {
+            *(u32x4*)dst[e] = x[e];
         }
-        bf16_t* dst = is_k ? p.k_out + (long)t * p.ko_st + (long)h * p.ko_sh : p.v_out + (long)t * p.vo_st + (long)h * p.vo_sh;
-        *(u32x4*)(dst + d0) = o;
     }
 }
 
@@ -250,21 +302,22 @@ MERV_DEVICE float sum_over_rows(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// tile at position tok (a multiple of 16): its halves lie in pages id0 and id1. `half1` is where the second half is read from: tok + 16, or tok again
-// where that is behind the row's last position
+struct PagedAt {  // where a tile's halves lie
+    int hkv, slot0, slot1, id0, id1;
+};
+
 template <int HD, bool E4M3>
-MERV_DEVICE void load_tile(PagedTile<HD, E4M3>& t, const PagedCacheArgs& c, int hkv, long tok, long half1, int id0, int id1) {
+MERV_DEVICE void load_tile(PagedTile<HD, E4M3>& t, const PagedCacheArgs& c, const PagedAt& at) {
     typedef PagedTile<HD, E4M3> Tile;
     constexpr int ELT = E4M3 ? 1 : 2;
     const int lane = threadIdx.x & 63, r = lane & 15, tg = lane >> 4;
-    const int mask = (1 << c.page_log2) - 1;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
-        const long id = tt ? id1 : id0;
-        const int slot = (int)((tt ? half1 : tok) & mask);
-        const long at = (id * c.s_page + (long)hkv * c.s_head + slot * c.s_tok) * ELT;
-        const char* kp = (const char*)c.k + at;
-        const char* vp = (const char*)c.v + at;
+        const long id = tt ? at.id1 : at.id0;
+        const int slot = tt ? at.slot1 : at.slot0;
+        const long off = (id * c.s_page + (long)at.hkv * c.s_head + slot * c.s_tok) * ELT;
+        const char* kp = (const char*)c.k + off;
+        const char* vp = (const char*)c.v + off;
         const unsigned krow = (unsigned)r * (unsigned)(c.s_tok * ELT) + tg * 16;
 #pragma unroll
         for (int j = 0; j < Tile::KL; ++j) t.k[tt][j] = *(const u32x4*)(kp + (krow + j * 64));
@@ -272,7 +325,7 @@ MERV_DEVICE void load_tile(PagedTile<HD, E4M3>& t, const PagedCacheArgs& c, int 
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words(t.v[tt * 4 + i], vp + i * c.s_tok * ELT + vrow);
         if constexpr (E4M3) {
-            const long sat = id * c.ss_page + (long)hkv * c.ss_head + slot;
+            const long sat = id * c.ss_page + (long)at.hkv * c.ss_head + slot;
             t.ks[tt] = *(const uint32_t*)(c.k_scale + sat + tg * 4);
             t.vs[tt] = *(const uint32_t*)(c.v_scale + sat + tg * 4);
         }
@@ -286,7 +339,7 @@ struct PagedState {  // of a wave: lane l has head l % 16
 };
 
 template <int HD, bool E4M3>
-MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, long tok, long lo, long len) {
+MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int tok, int lo, int len) {
     typedef PagedTile<HD, E4M3> Tile;
     const int lane = threadIdx.x & 63, tg = lane >> 4;
     f32x4 s[2];
@@ -315,7 +368,7 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const long j = tok + tt * 16 + tg * 4 + i;
+                const int j = tok + tt * 16 + tg * 4 + i;
                 const bool seen = j >= lo && j < len;
                 s[tt][i] = seen ? s[tt][i] : -INFINITY;
 #pragma unroll
@@ -377,132 +430,145 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
     }
 }
 
-// The units of `rows` rows, summed: thread t has those of rows t * per ... Returns the total; `before`: those of the rows before the thread's own.
-// Called by all 256 threads; scratch: 4 ints.
-MERV_DEVICE int scan_units(int mine, int& before, int* scratch) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    if (lane == 63) scratch[wave] = x;
-    __syncthreads();
-    int total = 0, under = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) under += scratch[w];
-        total += scratch[w];
-    }
-    before = under + x - mine;
-    return total;
+// over the lanes up to and with the own one
+MERV_DEVICE int wave_scan_add(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+MERV_DEVICE int wave_scan_max(int x) {  // of numbers that are not negative
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return x;
 }
 
+MERV_DEVICE PagedSpan span_of_len(const PagedAttnArgs& p, int len) { return paged_span(len, p.window, p.c.table_width << p.c.page_log2); }
+// of a row that is the same for the whole wave: through the scalar cache, which leaves the order of the vector loads (and the waits for them) alone
 MERV_DEVICE PagedSpan span_of(const PagedAttnArgs& p, int row) {
-    return paged_span(p.lens[row], p.window, (long)p.c.table_width << p.c.page_log2);
+    return span_of_len(p, *(const __attribute__((address_space(4))) int*)(uintptr_t)(p.lens + row));
+}
+
+// The workspace: a PagedOpen of each worker, then two partial sums (PAGED_HEAD_BLOCK heads of HD numbers, maximum, sum, 2 of padding) of each.
+struct PagedOpen {  // of the pair that begins in a worker and ends in a later one
+    int row, pair, slot, last;  // last: the worker that it ends in, -1: there is no such pair
+};
+template <int HD>
+MERV_DEVICE float* paged_sums(const PagedAttnArgs& p) {
+    return (float*)((PagedOpen*)p.ws + p.workers);
 }
 
 template <int HD>
 struct PagedLds {
-    float o[4][PAGED_HEAD_BLOCK][HD];
+    float o[4][PAGED_HEAD_BLOCK][HD + 4];  // (padded: heads lie in other banks)
     float m[4][PAGED_HEAD_BLOCK], l[4][PAGED_HEAD_BLOCK];
-    int scan[4], row, before;
 };
 
-// units u .. u + n - 1 of one pair, by the whole workgroup. slot < 0: all of the pair, the result is written.
+struct PagedSegment {  // units u .. u + n - 1 of one pair. slot < 0: all of the pair, the result is written.
+    int base, lo, len, units, row, pair, u, n, slot;
+};
+
+// What a wave holds of a segment: its tiles are 32 positions at first + 128 i, the pages of 32 of them at a time lie in `ids`, one half tile in each lane.
+struct PagedWalk {
+    int first, tiles, ids;
+};
+
+MERV_DEVICE int half_tile(const PagedSegment& g, int first, int t0) {  // the lane's one of 32 tiles from t0 on
+    const int lane = threadIdx.x & 63;
+    return min(first + (t0 + (lane >> 1)) * PAGED_UNIT + (lane & 1) * 16, g.len - 1);  // behind the row's end: the row's last position
+}
+MERV_DEVICE int load_ids(const PagedAttnArgs& p, const PagedSegment& g, int first, int t0) {
+    return (p.c.table + (long)g.row * p.c.table_stride)[half_tile(g, first, t0) >> p.c.page_log2];
+}
+
+// `pages`, where given: the row's pages, one in each lane
+template <bool GIVEN>
+MERV_DEVICE PagedWalk begin_walk(const PagedAttnArgs& p, const PagedSegment& g, int pages) {
+    PagedWalk w;
+    w.first = g.base + g.u * PAGED_UNIT + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
+    const int left = g.len - w.first;
+    w.tiles = left <= 0 || p.c.n_pages <= 0 ? 0 : min(g.n, (left + PAGED_UNIT - 1) / PAGED_UNIT);
+    if (GIVEN && p.c.table_width <= 64) w.ids = __shfl(pages, half_tile(g, w.first, 0) >> p.c.page_log2, 64);
+    else w.ids = load_ids(p, g, w.first, 0);
+    return w;
+}
+
+// page numbers that are none become page 0, and mark the segment
+MERV_DEVICE int checked_ids(const PagedAttnArgs& p, int ids, int& bad) {
+    const bool ok = ids >= 0 && ids < p.c.n_pages;
+    bad |= ok ? 0 : 1;
+    return ok ? ids : 0;
+}
+
+MERV_DEVICE PagedAt tile_at(const PagedAttnArgs& p, const PagedSegment& g, const PagedWalk& w, int i) {
+    const int tok = w.first + i * PAGED_UNIT, mask = (1 << p.c.page_log2) - 1;
+    const int half1 = tok + 16 < g.len ? tok + 16 : tok;  // behind the row's end: the first half again
+    return PagedAt{g.pair / p.head_blocks, tok & mask, half1 & mask, __builtin_amdgcn_readlane(w.ids, 2 * (i & 31)),
+                   __builtin_amdgcn_readlane(w.ids, 2 * (i & 31) + 1)};
+}
+
+// the queries of a segment's heads, as the second operand of S^T: lane l has head l % 16, the dims in the order in which its keys hold them
 template <int HD, bool E4M3>
-MERV_DEVICE void paged_segment(const PagedAttnArgs& p, PagedLds<HD>& lds, int row, int pair, const PagedSpan sp, int u, int n, int slot) {
+MERV_DEVICE void load_queries(bf16x8 (&q)[HD / 32], const PagedAttnArgs& p, const PagedSegment& g) {
+    const int lane = threadIdx.x & 63, group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
+    const int h0 = hkv * group + hb * PAGED_HEAD_BLOCK, heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
+    const bf16_t* qp = p.q + (long)g.row * p.q_st + (long)(h0 + min(lane & 15, heads - 1)) * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        const int d = E4M3 ? (j >> 1) * 64 + (lane >> 4) * 16 + (j & 1) * 8 : j * 32 + (lane >> 4) * 8;
+        q[j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + d));
+    }
+}
+
+// the four waves' sums of a segment, together: the result, or a partial sum
+template <int HD>
+MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD>& lds, const PagedSegment& g, PagedState<HD>& st, int bad) {
     constexpr int DV = HD / 16;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = p.H / p.c.kv_heads, blocks = p.head_blocks;
-    const int hkv = pair / blocks, hb = pair - hkv * blocks;
-    const int h0 = hkv * group + hb * PAGED_HEAD_BLOCK;
-    const int heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
-    // the first dims of a lane's keys: bf16 16 bytes of every 64; e4m3 16 codes of every 64
-    bf16x8 q[HD / 32];
-    {
-        const bf16_t* qp = p.q + (long)row * p.q_st + (long)(h0 + min(lane & 15, heads - 1)) * p.q_sh;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-            const int d = E4M3 ? (j >> 1) * 64 + (lane >> 4) * 16 + (j & 1) * 8 : j * 32 + (lane >> 4) * 8;
-            q[j] = __builtin_bit_cast(bf16x8, *(const u32x4*)(qp + d));
-        }
-    }
-    PagedState<HD> st;
-    st.m = -INFINITY;
-    st.l = 0.f;
-#pragma unroll
-    for (int d = 0; d < DV; ++d) st.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float scale2 = p.scale * LOG2E;
-    const int* table = p.c.table + (long)row * p.c.table_stride;
-    const long first = sp.base + (long)u * PAGED_UNIT + wave * 32;  // this wave's tiles: first + 128 i
-    const long left = sp.len - first;
-    const int tiles = left <= 0 ? 0 : min(n, (int)((left + PAGED_UNIT - 1) / PAGED_UNIT));
-    bool bad = false;
-    for (int t0 = 0; t0 < tiles; t0 += 32) {
-        // the pages of the next 32 tiles' halves, one in each lane; a half behind the row's end takes the page of the row's last position
-        long half = first + (long)(t0 + (lane >> 1)) * PAGED_UNIT + (lane & 1) * 16;
-        half = half < sp.len ? half : sp.len - 1;
-        int ids = table[half >> p.c.page_log2];
-        if (ids < 0 || ids >= p.c.n_pages) {
-            bad = true;
-            ids = 0;
-        }
-        const int end = min(32, tiles - t0);
-        const long tok0 = first + (long)t0 * PAGED_UNIT;
-        PagedTile<HD, E4M3> a, b;
-        auto load = [&](PagedTile<HD, E4M3>& t, int i) {
-            const long tok = tok0 + (long)i * PAGED_UNIT;
-            load_tile(t, p.c, hkv, tok, tok + 16 < sp.len ? tok + 16 : tok, __builtin_amdgcn_readlane(ids, 2 * i), __builtin_amdgcn_readlane(ids, 2 * i + 1));
-        };
-        auto use = [&](PagedTile<HD, E4M3>& t, int i) { use_tile(st, t, q, scale2, tok0 + (long)i * PAGED_UNIT, sp.lo, sp.len); };
-        if (p.c.n_pages > 0) {
-            load(a, 0);
-            for (int i = 0; i < end; i += 2) {
-                if (i + 1 < end) load(b, i + 1);
-                use(a, i);
-                if (i + 1 < end) {
-                    if (i + 2 < end) load(a, i + 2);
-                    use(b, i + 1);
-                }
-            }
-        }
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
+    const int h0 = hkv * group + hb * PAGED_HEAD_BLOCK, heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
     st.l = sum_over_rows(st.l);
     if (__any(bad)) st.l = __builtin_nanf("");
     const int h = lane & 15;
     if (h < heads) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            float* dst = &lds.o[wave][h][((lane >> 4) * 4 + i) * DV];
 #pragma unroll
-            for (int d = 0; d < DV; ++d) lds.o[wave][h][((lane >> 4) * 4 + i) * DV + d] = st.o[d][i];
+            for (int d = 0; d < DV; d += 4) *(f32x4*)(dst + d) = f32x4{st.o[d][i], st.o[d + 1][i], st.o[d + 2][i], st.o[d + 3][i]};
+        }
         if (lane < 16) {
             lds.m[wave][h] = st.m;
             lds.l[wave][h] = st.l;
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < heads * HD; e += 256) {
-        const int hh = e / HD, d = e % HD;
+    for (int e = threadIdx.x; e < heads * (HD / 4); e += 256) {
+        const int hh = e / (HD / 4), d = e % (HD / 4) * 4;
         const float M = fmaxf(fmaxf(lds.m[0][hh], lds.m[1][hh]), fmaxf(lds.m[2][hh], lds.m[3][hh])), base = M == -INFINITY ? 0.f : M;
-        float L = 0.f, O = 0.f;
+        float L = 0.f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float f = __builtin_amdgcn_exp2f(lds.m[w][hh] - base);
             L += f * lds.l[w][hh];
-            O += f * lds.o[w][hh][d];
+            O += f * *(const f32x4*)&lds.o[w][hh][d];
         }
-        if (slot < 0) {
-            p.out[(long)row * p.o_st + (long)(h0 + hh) * p.o_sh + d] = f2bf(O / L);
-            if (p.lse && d == 0) p.lse[(long)row * p.H + h0 + hh] = (M + __builtin_amdgcn_logf(L)) * LN2;
+        if (g.slot < 0) {
+            const u32x2 o = {pack2bf(O[0] / L, O[1] / L), pack2bf(O[2] / L, O[3] / L)};
+            *(u32x2*)(p.out + (long)g.row * p.o_st + (long)(h0 + hh) * p.o_sh + d) = o;
+            if (p.lse && d == 0) p.lse[(long)g.row * p.H + h0 + hh] = (M + __builtin_amdgcn_logf(L)) * LN2;
         } else {
-            float* ws = (float*)p.ws + ((size_t)slot * PAGED_HEAD_BLOCK + hh) * (HD + 4);
-            ws[d] = O;
-            if (d == 0) {
-                ws[HD] = M;
-                ws[HD + 1] = L;
-            }
+            float* ws = paged_sums<HD>(p) + ((size_t)g.slot * PAGED_HEAD_BLOCK + hh) * (HD + 4);
+            *(f32x4*)(ws + d) = O;
+            if (d == 0) *(f32x2*)(ws + HD) = f32x2{M, L};
         }
     }
     __syncthreads();
@@ -515,182 +581,353 @@ MERV_DEVICE void write_unseen(const PagedAttnArgs& p, int row, int h, int d) {  
     if (p.lse && d == 0) p.lse[(long)row * p.H + h] = p.lens[row] > 0 ? x : -INFINITY;
 }
 
-// DIRECT: a workgroup for each pair of each row, which writes the result. Else the line of units is shared out (paged_split.h).
+// what a worker leaves beside its sums: word of the pair that goes on behind it, and the results of every p.workers-th row that has no units
+template <int HD>
+MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
+    if (threadIdx.x == 0) ((PagedOpen*)p.ws)[blockIdx.x] = open;
+    for (int r = blockIdx.x; r < p.c.rows; r += p.workers)
+        if (span_of(p, r).units == 0)
+            for (int e = threadIdx.x; e < p.H * HD; e += 256) write_unseen<HD>(p, r, e / HD, e % HD);
+}
+
+// DIRECT: a workgroup for each pair of each row, which writes the result. Else the line of units is shared out, or, where the lengths are so, the pairs are
+// left whole as well (paged_split.h).
+//
+// One tile is always on its way: while a tile is used the next one is loaded, which behind a segment's last is the first of the workgroup's next segment
+// (whose pages were looked up a segment ahead). Behind the very last it is that one again, from the cache: a load that were left out there would make
+// the compiler wait, at each use, for the newer loads too. Lengths come through the scalar cache for the same reason.
+//
+// Bound by HBM where the call is large, by its chain of round trips (length, pages, keys and values, sums) where it is small. Measured, 128 dims:
+//   96 rows of 2458 .. 8192 positions, 32 / 8 heads, 16 bits: 354 us, 5.84 TB/s of keys and values (a copy of 1 GiB on this card: 5.05)
+//   1 row of 131072, 32 / 8 heads, 8 bits: 59 us, 4.55 TB/s, 8 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21 us, 2.9 TB/s
+//   1 row of 77, 16 / 2 heads: 4.6 us;  1 row of 1049, 32 / 32, 16 bits: 13.5 us, 3.9 of them the join
+// 512 workers: with 1024 the large call takes 363 us and 33 x 3001 takes a fifth more (twice the segments); with 256 half the loads are on their way.
+// Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit.
 template <int HD, bool E4M3, bool DIRECT>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p) {
     __shared__ PagedLds<HD> lds;
     const int pairs = p.c.kv_heads * p.head_blocks;
-    if constexpr (DIRECT) {
-        const int row = blockIdx.x / pairs, pair = blockIdx.x % pairs;
-        const PagedSpan sp = span_of(p, row);
-        if (sp.units > 0) {
-            paged_segment<HD, E4M3>(p, lds, row, pair, sp, 0, sp.units, -1);
+    PagedSegment g;
+    int x = 0, end = 0, w = 0;  // units of the line: behind this segment, behind this worker; the worker
+    PagedShare share{0, 0, 0};
+    PagedOpen open{0, 0, 0, -1};
+    int pages = 0;
+    bool whole = DIRECT;  // one pair of one row
+    if constexpr (!DIRECT) {
+        const int rows = p.c.rows, per = (rows + 63) / 64, lane = threadIdx.x & 63, r0 = min(rows, lane * per), r1 = min(rows, r0 + per);
+        int mine = 0, most = 0;
+        for (int r = r0; r < r1; ++r) {
+            const int n = span_of_len(p, p.lens[r]).units;
+            mine += n;
+            most = max(most, n);
+        }
+        const int sum = wave_scan_add(mine), total = __builtin_amdgcn_readlane(sum, 63) * pairs;
+        most = __builtin_amdgcn_readlane(wave_scan_max(most), 63);
+        whole = paged_whole(total, most, rows * pairs, gridDim.x);
+        w = blockIdx.x;
+        share = paged_share(total, p.workers);
+        if (whole) {
+            if (threadIdx.x == 0 && w < p.workers) ((PagedOpen*)p.ws)[w] = open;
+            if (w >= rows * pairs) return;
+        } else if (w >= share.workers) {
+            if (w < p.workers) end_worker<HD>(p, open);
+            return;
         } else {
-            const int group = p.H / p.c.kv_heads, hkv = pair / p.head_blocks, hb = pair % p.head_blocks;
-            const int heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
-            for (int e = threadIdx.x; e < heads * HD; e += 256) write_unseen<HD>(p, row, hkv * group + hb * PAGED_HEAD_BLOCK + e / HD, e % HD);
-        }
-    } else {
-        const int rows = p.c.rows, per = (rows + 255) / 256, r0 = min(rows, (int)threadIdx.x * per), r1 = min(rows, r0 + per);
-        int mine = 0, before = 0;
-        for (int r = r0; r < r1; ++r) mine += span_of(p, r).units;
-        const long total = (long)scan_units(mine, before, lds.scan) * pairs;
-        const int workers = paged_workers(total, gridDim.x), w = blockIdx.x;
-        if (w >= workers) return;
-        const long begin = paged_start(w, total, workers), end = paged_start(w + 1, total, workers);
-        if (begin >= (long)before * pairs && begin < (long)(before + mine) * pairs) {  // this thread's rows hold the first unit
-            int r = r0;
-            for (; r < r1; ++r) {
-                const int n = span_of(p, r).units;
-                if (begin < (long)(before + n) * pairs) break;
-                before += n;
+            x = paged_start(share, w);
+            end = paged_start(share, w + 1);
+            // the lane whose rows hold the first unit
+            const int at = __ffsll(__ballot(x >= (sum - mine) * pairs && x < sum * pairs)) - 1;
+            int before = __builtin_amdgcn_readlane(sum - mine, at);
+            g.row = at * per;
+            PagedSpan sp = span_of(p, g.row);
+            while (x >= (before + sp.units) * pairs) {
+                before += sp.units;
+                sp = span_of(p, ++g.row);
             }
-            lds.row = r;
-            lds.before = before;
-        }
-        __syncthreads();
-        int row = __builtin_amdgcn_readfirstlane(lds.row);
-        PagedSpan sp = span_of(p, row);
-        const long in_row = begin - (long)__builtin_amdgcn_readfirstlane(lds.before) * pairs;
-        int pair = (int)(in_row / sp.units), u = (int)(in_row % sp.units);
-        for (long x = begin; x < end;) {
-            const int n = (int)min((long)(sp.units - u), end - x);
-            paged_segment<HD, E4M3>(p, lds, row, pair, sp, u, n, n == sp.units ? -1 : x == begin ? 2 * w : 2 * w + 1);
-            x += n;
-            u = 0;
-            if (++pair == pairs && x < end) {
-                pair = 0;
-                do sp = span_of(p, ++row);
-                while (sp.units == 0);
-            }
+            g.base = sp.base, g.lo = sp.lo, g.len = sp.len, g.units = sp.units;
+            const int in_row = x - before * pairs;
+            g.pair = in_row / sp.units;
+            g.u = in_row - g.pair * sp.units;
+            g.n = min(g.units - g.u, end - x);
+            g.slot = g.n == g.units ? -1 : paged_slot(w, true);
+            if (g.u == 0 && g.n < g.units) open = PagedOpen{g.row, g.pair, g.slot, paged_owner(share, x + g.units - 1)};
+            x += g.n;
         }
     }
+    if (whole) {
+        g.row = blockIdx.x / pairs;
+        g.pair = blockIdx.x - g.row * pairs;
+        if constexpr (DIRECT) {  // a row's first 64 pages are requested together with its length
+            const int col = min((int)(threadIdx.x & 63), p.c.table_width - 1);
+            if (col >= 0) pages = (p.c.table + (long)g.row * p.c.table_stride)[col];
+        }
+        const PagedSpan sp = span_of(p, g.row);
+        if (sp.units == 0) {
+            const int group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
+            const int heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
+            for (int e = threadIdx.x; e < heads * HD; e += 256) write_unseen<HD>(p, g.row, hkv * group + hb * PAGED_HEAD_BLOCK + e / HD, e % HD);
+            return;
+        }
+        g.base = sp.base, g.lo = sp.lo, g.len = sp.len, g.units = sp.units;
+        g.u = 0, g.n = sp.units, g.slot = -1;
+    }
+    const float scale2 = p.scale * LOG2E;
+    PagedTile<HD, E4M3> a, b;
+    bf16x8 q[HD / 32];
+    int bad = 0;
+    PagedWalk walk = begin_walk<DIRECT>(p, g, pages);
+    load_queries<HD, E4M3>(q, p, g);
+    walk.ids = checked_ids(p, walk.ids, bad);
+    if (walk.tiles > 0) load_tile(a, p.c, tile_at(p, g, walk, 0));
+    for (;;) {
+        PagedSegment g2 = g;
+        PagedWalk walk2 = walk;
+        int bad2 = 0;
+        bool more = false;
+        if constexpr (!DIRECT) {
+            more = x < end;
+            if (more) {
+                g2.u = 0;
+                if (++g2.pair == pairs) {
+                    g2.pair = 0;
+                    PagedSpan sp;
+                    do sp = span_of(p, ++g2.row);
+                    while (sp.units == 0);
+                    g2.base = sp.base, g2.lo = sp.lo, g2.len = sp.len, g2.units = sp.units;
+                }
+                g2.n = min(g2.units, end - x);
+                g2.slot = g2.n == g2.units ? -1 : paged_slot(w, false);
+                if (g2.n < g2.units) open = PagedOpen{g2.row, g2.pair, g2.slot, paged_owner(share, x + g2.units - 1)};
+                x += g2.n;
+                walk2 = begin_walk<false>(p, g2, 0);
+            }
+        }
+        PagedState<HD> st;
+        st.m = -INFINITY;
+        st.l = 0.f;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) st.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // where the tile behind i lies
+        auto behind = [&](int i) {
+            if (i + 1 < walk.tiles) {
+                if (((i + 1) & 31) == 0) walk.ids = checked_ids(p, load_ids(p, g, walk.first, i + 1), bad);
+                return tile_at(p, g, walk, i + 1);
+            }
+            if (more && walk2.tiles > 0) {
+                walk2.ids = checked_ids(p, walk2.ids, bad2);
+                return tile_at(p, g2, walk2, 0);
+            }
+            return tile_at(p, g, walk, i);
+        };
+        bool in_b = false;  // the next segment's first tile
+        for (int i = 0; i < walk.tiles;) {
+            load_tile(b, p.c, behind(i));
+            __builtin_amdgcn_sched_barrier(0);  // all of the next tile is requested before the first wait for this one
+            use_tile(st, a, q, scale2, walk.first + i * PAGED_UNIT, g.lo, g.len);
+            if (++i == walk.tiles) {
+                in_b = true;
+                break;
+            }
+            load_tile(a, p.c, behind(i));
+            __builtin_amdgcn_sched_barrier(0);
+            use_tile(st, b, q, scale2, walk.first + i * PAGED_UNIT, g.lo, g.len);
+            ++i;
+        }
+        if (more) {
+            load_queries<HD, E4M3>(q, p, g2);
+            if (walk.tiles == 0 && walk2.tiles > 0) {  // else it is on its way
+                walk2.ids = checked_ids(p, walk2.ids, bad2);
+                load_tile(a, p.c, tile_at(p, g2, walk2, 0));
+            }
+        }
+        end_segment(p, lds, g, st, bad);
+        if (!more) break;
+        if (in_b) a = b;
+        g = g2;
+        walk = walk2;
+        walk.ids = checked_ids(p, walk.ids, bad2);
+        bad = bad2;
+    }
+    if constexpr (!DIRECT)
+        if (!whole) end_worker<HD>(p, open);
 }
 
-// one workgroup for a row and a query head: the partial sums of its pair, 256 / HD of them at a time
+// Joins the partial sums of the pair that begins in a worker and ends in a later one, if there is one; the worker left word of it (PagedOpen), so nothing
+// about the lengths is worked out again. A workgroup for a worker and a head. Up to JOIN_MANY sums: the first of four heads' workgroups takes all four, a
+// wave each. More: each takes its own, wave w the workers w, w + 4 .. behind the first, and the four meet in LDS.
+constexpr int JOIN_MANY = 16;
+
+template <int HD>
+struct PagedSum {
+    float m, l, o[HD / 64];
+};
+
+// EACH sums are requested at a time (behind the last one, that one again: a load that is left out would keep the others from going out together)
+template <int HD, int EACH>
+MERV_DEVICE PagedSum<HD> join_sums(const float* sums, const PagedOpen& open, int w0, int hh, int from, int step) {
+    constexpr int DPL = HD / 64;
+    const int lane = threadIdx.x & 63;
+    PagedSum<HD> s{-INFINITY, 0.f, {}};
+    for (int w = w0 + from; w <= open.last; w += step * EACH) {
+        f32x2 ml[EACH];
+        float o[EACH][DPL];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int v = min(w + step * e, open.last);
+            const float* x = sums + ((size_t)(v == w0 ? open.slot : 2 * v) * PAGED_HEAD_BLOCK + hh) * (HD + 4);
+            ml[e] = *(const f32x2*)(x + HD);
+            if constexpr (DPL == 2) {
+                const f32x2 y = *(const f32x2*)(x + lane * 2);
+                o[e][0] = y[0], o[e][1] = y[1];
+            } else {
+                o[e][0] = x[lane];
+            }
+        }
+        float top = s.m;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            asm volatile("" : "+v"(ml[e]));  // (here, so that no load sinks to its use)
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) asm volatile("" : "+v"(o[e][d]));
+            top = fmaxf(top, ml[e][0]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, a = __builtin_amdgcn_exp2f(s.m - base);
+        s.m = top;
+        s.l *= a;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) s.o[d] *= a;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const bool on = w + step * e <= open.last;
+            const float f = __builtin_amdgcn_exp2f(ml[e][0] - base);
+            s.l += on ? f * ml[e][1] : 0.f;
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) s.o[d] += on ? f * o[e][d] : 0.f;
+        }
+    }
+    return s;
+}
+
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs p) {
-    constexpr int PARTS = 256 / HD;
-    __shared__ int scan[4], found;
-    __shared__ float sm[PARTS][2], so[PARTS][HD];
-    const int row = blockIdx.x / p.H, h = blockIdx.x % p.H, pairs = p.c.kv_heads * p.head_blocks;
-    const int rows = p.c.rows, per = (rows + 255) / 256, r0 = min(rows, (int)threadIdx.x * per), r1 = min(rows, r0 + per);
-    int mine = 0, before = 0;
-    for (int r = r0; r < r1; ++r) mine += span_of(p, r).units;
-    const long total = (long)scan_units(mine, before, scan) * pairs;
-    if (row >= r0 && row < r1) {
-        for (int r = r0; r < row; ++r) before += span_of(p, r).units;
-        found = before;
-    }
-    __syncthreads();
-    const int part = threadIdx.x / HD, d = threadIdx.x % HD;
-    const int units = span_of(p, row).units;
-    if (units == 0) {
-        if (part == 0) write_unseen<HD>(p, row, h, d);
-        return;
-    }
-    const int group = p.H / p.c.kv_heads, hkv = h / group, hb = (h % group) / PAGED_HEAD_BLOCK, hh = (h % group) % PAGED_HEAD_BLOCK;
-    const long first = (long)found * pairs + (long)(hkv * p.head_blocks + hb) * units;
-    const int workers = paged_workers(total, p.workers);
-    const int w0 = paged_owner(first, total, workers), w1 = paged_owner(first + units - 1, total, workers);
-    if (w0 == w1) return;  // written by its worker
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = w0 + part; w <= w1; w += PARTS) {
-        const float* ws = (const float*)p.ws + ((size_t)paged_slot(w, first, total, workers) * PAGED_HEAD_BLOCK + hh) * (HD + 4);
-        const float m = ws[HD], l = ws[HD + 1], o = ws[d];
-        const float top = fmaxf(M, m), base = top == -INFINITY ? 0.f : top;
-        const float a = __builtin_amdgcn_exp2f(M - base), b = __builtin_amdgcn_exp2f(m - base);
-        L = L * a + l * b;
-        O = O * a + o * b;
-        M = top;
-    }
-    so[part][d] = O;
-    if (d == 0) {
-        sm[part][0] = M;
-        sm[part][1] = L;
-    }
-    __syncthreads();
-    if (part) return;
-    float top = -INFINITY;
+    constexpr int DPL = HD / 64;
+    __shared__ float sm[4], sl[4], so[4][HD];
+    const PagedOpen open = ((const PagedOpen*)p.ws)[blockIdx.x];
+    const int w0 = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool few = open.last - w0 < JOIN_MANY;
+    if (open.last < 0 || (few && (blockIdx.y & 3))) return;
+    const int group = p.H / p.c.kv_heads, hkv = open.pair / p.head_blocks, hb = open.pair - hkv * p.head_blocks;
+    const int hh = few ? blockIdx.y + wave : blockIdx.y, h = hkv * group + hb * PAGED_HEAD_BLOCK + hh;
+    if (hb * PAGED_HEAD_BLOCK + hh >= group || hh >= PAGED_HEAD_BLOCK) return;  // (not few: the whole workgroup)
+    PagedSum<HD> s;
+    if (few) {
+        s = join_sums<HD, 4>(paged_sums<HD>(p), open, w0, hh, 0, 1);
+    } else {
+        s = join_sums<HD, JOIN_MANY>(paged_sums<HD>(p), open, w0, hh, wave, 4);
+        if (lane == 0) {
+            sm[wave] = s.m;
+            sl[wave] = s.l;
+        }
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) top = fmaxf(top, sm[i][0]);
-    const float base = top == -INFINITY ? 0.f : top;
-    L = O = 0.f;
+        for (int d = 0; d < DPL; ++d) so[wave][lane * DPL + d] = s.o[d];
+        __syncthreads();
+        if (wave) return;
+        const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), base = top == -INFINITY ? 0.f : top;
+        s = PagedSum<HD>{top, 0.f, {}};
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-        const float f = __builtin_amdgcn_exp2f(sm[i][0] - base);
-        L += f * sm[i][1];
-        O += f * so[i][d];
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sm[w] - base);
+            s.l += f * sl[w];
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) s.o[d] += f * so[w][lane * DPL + d];
+        }
     }
-    p.out[(long)row * p.o_st + (long)h * p.o_sh + d] = f2bf(O / L);
-    if (p.lse && d == 0) p.lse[(long)row * p.H + h] = (top + __builtin_amdgcn_logf(L)) * LN2;
+    bf16_t* out = p.out + (long)open.row * p.o_st + (long)h * p.o_sh + lane * DPL;
+    if constexpr (DPL == 2) *(uint32_t*)out = pack2bf(s.o[0] / s.l, s.o[1] / s.l);
+    else *out = f2bf(s.o[0] / s.l);
+    if (p.lse && lane == 0) p.lse[(long)open.row * p.H + h] = (s.m + __builtin_amdgcn_logf(s.l)) * LN2;
 }
 
 }  // namespace
 
+// EACH vectors for each group of lanes: as many as still leave the card two workgroups a CU or more
+template <int HD, bool E4M3, int EACH>
+static void launch_paged_write_each(const PagedWriteArgs& a, long vectors, hipStream_t s) {
+    const long each = 256 / (HD / 16) * EACH;
+    hipLaunchKernelGGL((paged_write_kernel<HD, E4M3, EACH>), dim3((unsigned)((vectors + each - 1) / each)), dim3(256), 0, s, a);
+}
+template <int HD, bool E4M3>
+static void launch_paged_write_as(const PagedWriteArgs& a, hipStream_t s) {
+    const long vectors = (long)a.T * (2 * a.c.kv_heads + a.H);
+    if (vectors >= 512L * 2 * 256 / (HD / 16)) launch_paged_write_each<HD, E4M3, 2>(a, vectors, s);
+    else launch_paged_write_each<HD, E4M3, 1>(a, vectors, s);
+}
+
 hipError_t launch_paged_write(const PagedWriteArgs& a, hipStream_t s) {
     if (a.T <= 0) return hipSuccess;
-    const dim3 grid((unsigned)a.T), block(256);
-    if (a.c.hd == 128) {
-        if (a.c.e4m3) hipLaunchKernelGGL((paged_write_kernel<128, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_write_kernel<128, false>), grid, block, 0, s, a);
-    } else if (a.c.hd == 64) {
-        if (a.c.e4m3) hipLaunchKernelGGL((paged_write_kernel<64, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_write_kernel<64, false>), grid, block, 0, s, a);
-    } else {
-        return hipErrorInvalidValue;
-    }
+    if (a.c.hd == 128) a.c.e4m3 ? launch_paged_write_as<128, true>(a, s) : launch_paged_write_as<128, false>(a, s);
+    else if (a.c.hd == 64) a.c.e4m3 ? launch_paged_write_as<64, true>(a, s) : launch_paged_write_as<64, false>(a, s);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
+}
+
+template <int HD, bool E4M3, int EACH>
+static void launch_paged_read_each(const PagedReadArgs& a, long vectors, hipStream_t s) {
+    const long each = 256 / (E4M3 ? HD / 16 : HD / 8) * EACH;
+    hipLaunchKernelGGL((paged_read_kernel<HD, E4M3, EACH>), dim3((unsigned)((vectors + each - 1) / each)), dim3(256), 0, s, a);
+}
+template <int HD, bool E4M3>
+static void launch_paged_read_as(const PagedReadArgs& a, hipStream_t s) {
+    const long vectors = (long)a.T * 2 * a.c.kv_heads;
+    if (vectors >= 512L * 4 * 256 / (E4M3 ? HD / 16 : HD / 8)) launch_paged_read_each<HD, E4M3, 4>(a, vectors, s);
+    else launch_paged_read_each<HD, E4M3, 1>(a, vectors, s);
 }
 
 hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s) {
     if (a.T <= 0) return hipSuccess;
-    const dim3 grid((unsigned)a.T), block(256);
-    if (a.c.hd == 128) {
-        if (a.c.e4m3) hipLaunchKernelGGL((paged_read_kernel<128, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_read_kernel<128, false>), grid, block, 0, s, a);
-    } else if (a.c.hd == 64) {
-        if (a.c.e4m3) hipLaunchKernelGGL((paged_read_kernel<64, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((paged_read_kernel<64, false>), grid, block, 0, s, a);
-    } else {
-        return hipErrorInvalidValue;
-    }
+    if (a.c.hd == 128) a.c.e4m3 ? launch_paged_read_as<128, true>(a, s) : launch_paged_read_as<128, false>(a, s);
+    else if (a.c.hd == 64) a.c.e4m3 ? launch_paged_read_as<64, true>(a, s) : launch_paged_read_as<64, false>(a, s);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
-// What a call launches, from sizes alone (the rows' lengths are on the device): up to DIRECT_UNITS units a row, one workgroup for each pair takes the
-// whole row and there is no join.
-constexpr long DIRECT_UNITS = 4;
+// What a call launches, from sizes alone (the rows' lengths are on the device). Where a row cannot be long, one workgroup for each pair takes it whole and
+// there is no join: up to 6 units, or 16 where there are pairs enough to fill half the card (then the longest possible row costs 22 us).
+// Measured, 16 bits, 128 dims, this and the split one: 5 units, 1 x 32 pairs 9.0 and 10.1 us, 33 x 4 9.6 and 18.1 us; 9 units, 1 x 8 13.2 and 9.7 us, 33 x 4 14.2 and
+// 17.5 us; 16 units, 33 x 4 21.9 and 23.8 us, 8 x 8 21.7 and 16.6 us.
+static bool paged_direct(long units, long pairs) { return units <= 6 || (units <= 16 && pairs >= 128); }
 
 struct PagedPlan {
-    int head_blocks, workers;
+    int head_blocks, workers, grid;
     bool direct;
 };
 static PagedPlan paged_plan(int rows, int H, int kv_heads, long capacity) {
     PagedPlan pl;
     pl.head_blocks = (H / kv_heads + PAGED_HEAD_BLOCK - 1) / PAGED_HEAD_BLOCK;
     const long units = (capacity + PAGED_UNIT - 1) / PAGED_UNIT;
-    const long most = units * rows * kv_heads * pl.head_blocks;
-    pl.direct = units <= DIRECT_UNITS;
+    const long pairs = (long)rows * kv_heads * pl.head_blocks, most = units * pairs;
     pl.workers = (int)(most < PAGED_MAX_WORKERS ? most : PAGED_MAX_WORKERS);
+    pl.direct = paged_direct(units, pairs);
+    pl.grid = (int)(pl.direct || (pairs > pl.workers && pairs <= PAGED_MOST_WHOLE) ? pairs : pl.workers);
     return pl;
 }
 
 size_t paged_attention_workspace_bytes(int rows, int H, int kv_heads, int hd, long capacity) {
     const PagedPlan pl = paged_plan(rows, H, kv_heads, capacity);
-    return pl.direct ? 0 : (size_t)2 * pl.workers * PAGED_HEAD_BLOCK * (hd + 4) * sizeof(float);
+    return pl.direct ? 0 : pl.workers * (sizeof(PagedOpen) + (size_t)2 * PAGED_HEAD_BLOCK * (hd + 4) * sizeof(float));
 }
 
 template <int HD, bool E4M3>
-static hipError_t launch_paged_attention_as(const PagedAttnArgs& a, bool direct, hipStream_t s) {
-    if (direct) {
-        hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, true>), dim3((unsigned)(a.c.rows * a.c.kv_heads * a.head_blocks)), dim3(256), 0, s, a);
+static hipError_t launch_paged_attention_as(const PagedAttnArgs& a, const PagedPlan& pl, hipStream_t s) {
+    if (pl.direct) {
+        hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, true>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, false>), dim3((unsigned)a.workers), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, false>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((paged_join_kernel<HD>), dim3((unsigned)(a.c.rows * a.H)), dim3(256), 0, s, a);
+    const int group = a.H / a.c.kv_heads;
+    hipLaunchKernelGGL((paged_join_kernel<HD>), dim3((unsigned)a.workers, (unsigned)(group < PAGED_HEAD_BLOCK ? group : PAGED_HEAD_BLOCK)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -700,8 +937,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, hipStream_t s) {
     const PagedPlan pl = paged_plan(a.c.rows, a.H, a.c.kv_heads, (long)a.c.table_width << a.c.page_log2);
     a.head_blocks = pl.head_blocks;
     a.workers = pl.workers;
-    if (a.c.hd == 128) return a.c.e4m3 ? launch_paged_attention_as<128, true>(a, pl.direct, s) : launch_paged_attention_as<128, false>(a, pl.direct, s);
-    if (a.c.hd == 64) return a.c.e4m3 ? launch_paged_attention_as<64, true>(a, pl.direct, s) : launch_paged_attention_as<64, false>(a, pl.direct, s);
+    if (a.c.hd == 128) return a.c.e4m3 ? launch_paged_attention_as<128, true>(a, pl, s) : launch_paged_attention_as<128, false>(a, pl, s);
+    if (a.c.hd == 64) return a.c.e4m3 ? launch_paged_attention_as<64, true>(a, pl, s) : launch_paged_attention_as<64, false>(a, pl, s);
     return hipErrorInvalidValue;
 }
 

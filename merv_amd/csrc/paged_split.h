@@ -5,9 +5,10 @@
 // stretch of the line, all stretches of the same length but for one unit, so rows of any lengths load the card evenly. A stretch is cut into segments
 // where a pair ends; a segment that is all of its pair writes the result, any other one leaves a partial sum: a worker has at most two, its
 // first and its last segment. The partial sums of a pair are joined in the workers' order, which depends on the lengths alone.
+// All numbers fit 31 bits (the entry point refuses larger calls), so that the divisions are 32-bit ones.
 #pragma once
 #ifdef __HIPCC__
-#define MERV_HD __host__ __device__ inline
+#define MERV_HD __host__ __device__ __forceinline__
 #else
 #define MERV_HD inline
 #endif
@@ -19,24 +20,45 @@ constexpr int PAGED_HEAD_BLOCK = 16;   // query heads of one workgroup: the colu
 constexpr int PAGED_MAX_WORKERS = 512; // two workgroups on each of 256 CUs
 
 struct PagedSpan {
-    long base, lo, len;  // units count from `base`; positions lo <= j < len are seen
-    int units;
+    int base, lo, len, units;  // units count from `base`; positions lo <= j < len are seen
 };
-// a length that is not positive, or over the capacity, has no units (the join writes such rows)
-MERV_HD PagedSpan paged_span(long len, long window, long capacity) {
+// a length that is not positive, or over the capacity, has no units (such rows are written apart); window 0: none
+MERV_HD PagedSpan paged_span(int len, int window, int capacity) {
     PagedSpan s{0, 0, len, 0};
     if (len <= 0 || len > capacity) return s;
     s.lo = window > 0 && len > window ? len - window : 0;
-    s.base = s.lo & ~15L;
-    s.units = (int)((len - s.base + PAGED_UNIT - 1) / PAGED_UNIT);
+    s.base = s.lo & ~15;
+    s.units = (len - s.base + PAGED_UNIT - 1) / PAGED_UNIT;
     return s;
 }
 
-// `total` units on the line, `workers` workers at most: each has one unit or more
-MERV_HD int paged_workers(long total, int workers) { return total < workers ? (int)total : workers; }
-MERV_HD long paged_start(int w, long total, int workers) { return total * w / workers; }
-MERV_HD int paged_owner(long unit, long total, int workers) { return (int)(((unit + 1) * workers - 1) / total); }
-// the partial sum that worker w leaves of the pair whose units begin at `first`: slot 2w if the pair is in its first segment, 2w + 1 if in its last
-MERV_HD int paged_slot(int w, long first, long total, int workers) { return 2 * w + (paged_start(w, total, workers) < first ? 1 : 0); }
+// `total` units on the line for `most` workers: the first `more` have each + 1 of them, the others each, and where there are fewer units than workers
+// the last have none
+struct PagedShare {
+    int workers, each, more;
+};
+MERV_HD PagedShare paged_share(int total, int most) {
+    const int workers = total < most ? total : most;
+    if (workers <= 0) return PagedShare{0, 0, 0};
+    return PagedShare{workers, total / workers, total % workers};
+}
+MERV_HD int paged_start(const PagedShare& s, int w) { return w * s.each + (w < s.more ? w : s.more); }
+MERV_HD int paged_owner(const PagedShare& s, int unit) {
+    const int long_ones = s.more * (s.each + 1);
+    return unit < long_ones ? unit / (s.each + 1) : s.more + (unit - long_ones) / s.each;
+}
+// Whether each pair of each row is left whole, a workgroup for each of the `all` pairs and nothing to join. A pair alone on its CU takes about a quarter of the
+// time for a unit that the fully loaded card needs for one more unit for each of its workers, and splitting costs four to five such quarters (workers
+// change rows, sums are joined): so no pair may be longer than that buys. Fewer than 512 pairs leave part of the card's bandwidth unused, which
+// counts once there are more than three units for each worker. Measured, 8-bit, 128 dims: 64 x 8 pairs of up to 9 units 23.0 us whole, 27.2 split; 33 x 4 of up
+// to 9: 16.0 and 20.9; 64 dims, 16 bits: 24 x 12 of 8 units: 20.9 and 19.1.
+constexpr int PAGED_MOST_WHOLE = 4096;
+MERV_HD bool paged_whole(int total, int most, int all, int grid) {
+    if (all > grid || all < 128 || most > 24 || (most - 4) * 128 > total) return false;
+    return all >= PAGED_MAX_WORKERS || total <= 3 * PAGED_MAX_WORKERS;
+}
+// A worker's partial sums: slot 2w is its first segment's, 2w + 1 its last one's where that is another. All workers of a pair but the one it begins in leave
+// its sum in 2w.
+MERV_HD int paged_slot(int w, bool first_segment) { return 2 * w + (first_segment ? 0 : 1); }
 
 }  // namespace merv

@@ -5,6 +5,7 @@ All tensors must be contiguous CUDA (ROCm) tensors: bf16 activations / GEMM weig
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -147,50 +148,65 @@ def gemm_mxfp8(aq, a_sc, wq, w_sc, bias=None, act="none", lscale=None, res=None,
 # standing for code * 2^(byte - 127)); table [rows, width] int32 names the page of positions i * page_size .. of a row. Any strides, last
 # dimension contiguous. Row lengths, offsets and page numbers stay on the device (a captured step replays with new ones); the kernels check
 # them: see include/merv_hip.h for what a bad one does. All of this is for inference: no gradients.
-def _stride(t: torch.Tensor, i: int) -> int:
-    return t.stride(i) if t.shape[i] > 1 else 0  # the stride of a dimension of one means nothing
+# These calls are made once a layer and token, so their checks read each attribute of a tensor once and build the C structure in one step.
+_PAGED_CACHE = struct.Struct("@5P7q6i")  # merv_paged_cache
 
 
-def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales) -> PagedCache:
-    if k_pages.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or k_pages.dim() != 4 or not k_pages.is_cuda:
+def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written: bool = False):
+    """-> (the C structure, device, rows, kv_heads, head_dim, positions that a row's table can hold)."""
+    kind, shape, dev = k_pages.dtype, k_pages.shape, k_pages.device
+    if kind not in (torch.bfloat16, torch.float8_e4m3fn) or len(shape) != 4 or dev.type != "cuda":
         raise ValueError(f"{what}: expected CUDA pages [n_pages, kv_heads, page_size, head_dim] of bfloat16 or float8_e4m3fn, got "
-                         f"{k_pages.dtype} {tuple(k_pages.shape)} on {k_pages.device}")
-    n_pages, kv_heads, page, hd = k_pages.shape
-    dev, e4m3 = k_pages.device, k_pages.dtype != torch.bfloat16
-    if v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride() or v_pages.device != dev:
+                         f"{kind} {tuple(shape)} on {dev}")
+    st = k_pages.stride()
+    if v_pages.dtype != kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.device != dev:
         raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
-    if k_pages.stride(3) != 1:
+    n_pages, kv_heads, page, hd = shape
+    if st[3] != 1:
         raise ValueError(f"{what}: the pages' last dimension must be contiguous")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
+    rows, width = table.shape if table.dim() == 2 else (-1, -1)
+    tst = table.stride()
+    if rows < 0 or table.dtype != torch.int32 or table.device != dev or (tst[1] != 1 and width > 1):
         raise ValueError(f"{what}: expected an int32 table [rows, width] on {dev} with contiguous rows")
-    ss_page = ss_head = 0
-    if e4m3:
+    ks = vs = 0
+    sst = (0, 0)
+    if kind != torch.bfloat16:
         if k_scales is None or v_scales is None:
             raise ValueError(f"{what}: float8_e4m3fn pages need k_scales and v_scales")
-        for s in (k_scales, v_scales):
-            if s.dtype != torch.uint8 or s.shape != k_pages.shape[:3] or s.device != dev or s.stride(2) != 1 or s.stride() != k_scales.stride():
-                raise ValueError(f"{what}: expected uint8 scales {tuple(k_pages.shape[:3])} on {dev}, tokens contiguous, of the same strides")
-        ss_page, ss_head = _stride(k_scales, 0), _stride(k_scales, 1)
+        sst = k_scales.stride()
+        for x in (k_scales, v_scales):
+            if x.dtype != torch.uint8 or x.shape != shape[:3] or x.device != dev or x.stride() != sst or sst[2] != 1:
+                raise ValueError(f"{what}: expected uint8 scales {tuple(shape[:3])} on {dev}, tokens contiguous, of the same strides")
+        ks, vs = k_scales.data_ptr(), v_scales.data_ptr()
+        if written and (sst[0] == 0 and n_pages > 1 or sst[1] == 0 and kv_heads > 1):
+            raise ValueError(f"{what}: scales that are written must not share memory")
     elif k_scales is not None or v_scales is not None:
         raise ValueError(f"{what}: bfloat16 pages take no scales")
-    return PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr() if e4m3 else 0, v_scales.data_ptr() if e4m3 else 0, table.data_ptr(),
-                      n_pages, _stride(k_pages, 0), _stride(k_pages, 1), _stride(k_pages, 2), ss_page, ss_head, _stride(table, 0), table.shape[0],
-                      table.shape[1], kv_heads, hd, page, KV_E4M3 if e4m3 else KV_BF16)
+    if written and (st[0] == 0 and n_pages > 1 or st[1] == 0 and kv_heads > 1 or st[2] == 0):
+        raise ValueError(f"{what}: pages that are written must not share memory")
+    # the stride of a dimension of one means nothing: 0
+    c = PagedCache.from_buffer_copy(_PAGED_CACHE.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), n_pages, st[0] if n_pages > 1 else 0, st[1] if kv_heads > 1 else 0, st[2],
+        sst[0] if n_pages > 1 else 0, sst[1] if kv_heads > 1 else 0, tst[0] if rows > 1 else 0, rows, width, kv_heads, hd, page,
+        KV_BF16 if kind == torch.bfloat16 else KV_E4M3))
+    return c, dev, rows, kv_heads, hd, width * page
 
 
 def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev, out: bool = False):
-    if t.dtype != torch.bfloat16 or t.shape != shape or t.device != dev or t.stride(2) != 1:
+    st = t.stride()
+    if t.dtype != torch.bfloat16 or t.shape != shape or t.device != dev or st[2] != 1:
         raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on {dev} with contiguous last dimension, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
-    if out and (t.stride(0) == 0 and shape[0] > 1 or t.stride(1) == 0 and shape[1] > 1):
+    s0, s1 = st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0
+    if out and (s0 == 0 and shape[0] > 1 or s1 == 0 and shape[1] > 1):
         raise ValueError(f"{what}: {name}: an output's rows must not share memory")
-    return t.data_ptr(), _stride(t, 0), _stride(t, 1)
+    return t.data_ptr(), s0, s1
 
 
 def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != dev or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != dev or (t.stride(0) != 1 and n > 1):
         raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -198,10 +214,12 @@ def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev) ->
 def _launch_on(dev, call, what: str, *args) -> None:
     """call(*args, stream) on the device's current stream; the device is made current where it is not (its null stream has no device of its own)."""
     if torch.cuda.current_device() == dev.index:
-        check(call(*args, current_stream_ptr(dev)), what)
+        rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
     else:
         with torch.cuda.device(dev):
-            check(call(*args, current_stream_ptr(dev)), what)
+            rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, what)
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
@@ -214,38 +232,38 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     the rotated queries (q_out, or a new tensor; q_out=q rotates in place), None without q; k_out takes the rotated keys as well. float8_e4m3fn pages:
     quantised with one power-of-two scale for each token and head (k_scales, v_scales); what is not finite becomes NaN."""
     what = "paged_cache_write"
-    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
-    for t in (k_pages, k_scales):
-        if t is not None and any(t.stride(i) == 0 and t.shape[i] > 1 for i in range(3)):
-            raise ValueError(f"{what}: pages and scales must not share memory among themselves")
-    dev = k_pages.device
+    cache, dev, rows, kv_heads, hd, _ = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales, True)
     if k.dim() != 3:
         raise ValueError(f"{what}: k: expected [tokens, kv_heads, head_dim], got {tuple(k.shape)}")
-    T, shape = k.shape[0], (k.shape[0], cache.kv_heads, cache.head_dim)
-    if offsets is None and T != cache.rows:
-        raise ValueError(f"{what}: without offsets there is one token for each row: {T} tokens, {cache.rows} rows")
+    T = k.shape[0]
+    shape = (T, kv_heads, hd)
+    if offsets is None and T != rows:
+        raise ValueError(f"{what}: without offsets there is one token for each row: {T} tokens, {rows} rows")
     kr, vr = _paged_rows(what, "k", k, shape, dev), _paged_rows(what, "v", v, shape, dev)
-    off_p, start_p = _paged_ints(what, "offsets", offsets, cache.rows + 1, dev), _paged_ints(what, "start", start, cache.rows, dev)
-    if (cos is None) != (sin is None) or (q is not None and cos is None) or (q_out is not None and q is None):
-        raise ValueError(f"{what}: cos and sin come together, q needs them, and q_out needs q")
-    rope = (0, 0, 0, 0)
-    if cos is not None:
+    off_p, start_p = _paged_ints(what, "offsets", offsets, rows + 1, dev), _paged_ints(what, "start", start, rows, dev)
+    rope, heads, qr, qo, ko = (0, 0, 0, 0), 0, (0, 0, 0), (0, 0, 0), (0, 0, 0)
+    if cos is not None and sin is not None:
+        cst, cshape = cos.stride(), cos.shape
         for t in (cos, sin):
-            if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != cache.head_dim or t.device != dev \
-                    or t.stride(1) != 1 or t.stride() != cos.stride():
-                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {cache.head_dim}] on {dev} with contiguous rows, of the same strides")
-        rope = (cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else cos.shape[1])
-    heads, qr, qo = 0, (0, 0, 0), (0, 0, 0)
+            if t.dtype != torch.bfloat16 or t.shape != cshape or len(cshape) != 2 or cshape[1] != hd or t.device != dev or t.stride() != cst or cst[1] != 1:
+                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {hd}] on {dev} with contiguous rows, of the same strides")
+        rope = (cos.data_ptr(), sin.data_ptr(), cshape[0], cst[0] if cshape[0] > 1 else hd)
+    elif cos is not None or sin is not None or q is not None:
+        raise ValueError(f"{what}: cos and sin come together, and q needs them")
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != cache.head_dim:
-            raise ValueError(f"{what}: q: expected [{T}, heads, {cache.head_dim}], got {tuple(q.shape)}")
-        heads = q.shape[1]
-        qr = _paged_rows(what, "q", q, q.shape, dev)
+        qshape = q.shape
+        if len(qshape) != 3 or qshape[0] != T or qshape[2] != hd:
+            raise ValueError(f"{what}: q: expected [{T}, heads, {hd}], got {tuple(qshape)}")
+        heads = qshape[1]
+        qr = _paged_rows(what, "q", q, qshape, dev)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        qo = _paged_rows(what, "q_out", q_out, q.shape, dev, True)
-    ko = _paged_rows(what, "k_out", k_out, shape, dev, True) if k_out is not None else (0, 0, 0)
-    _launch_on(dev, _lib.load().merv_paged_cache_write, "merv_paged_cache_write", cache, *kr, *vr, *qr, *rope, *qo, *ko, off_p, start_p, T, heads)
+            q_out = q.new_empty(qshape)
+        qo = _paged_rows(what, "q_out", q_out, qshape, dev, True)
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out needs q")
+    if k_out is not None:
+        ko = _paged_rows(what, "k_out", k_out, shape, dev, True)
+    _launch_on(dev, _lib.load().merv_paged_cache_write, what, cache, *kr, *vr, *qr, *rope, *qo, *ko, off_p, start_p, T, heads)
     return q_out
 
 
@@ -256,17 +274,18 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.
     (start[b] or 0) + t - offsets[b] where offsets[b] <= t < offsets[b + 1]. Outputs behind offsets[rows], and those of rows with start[b] < 0, are
     not written. A position without a page reads as NaN. Numbers are given back exactly as the cache holds them."""
     what = "paged_cache_read"
-    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
-    dev, shape = k_pages.device, (int(total), cache.kv_heads, cache.head_dim)
+    cache, dev, rows, kv_heads, hd, _ = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
+    total = int(total)
     if total < 0 or offsets is None:
         raise ValueError(f"{what}: total must not be negative, and offsets are needed")
-    off_p, start_p = _paged_ints(what, "offsets", offsets, cache.rows + 1, dev), _paged_ints(what, "start", start, cache.rows, dev)
+    shape = (total, kv_heads, hd)
+    off_p, start_p = _paged_ints(what, "offsets", offsets, rows + 1, dev), _paged_ints(what, "start", start, rows, dev)
     if k_out is None:
         k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     if v_out is None:
         v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
     ko, vo = _paged_rows(what, "k_out", k_out, shape, dev, True), _paged_rows(what, "v_out", v_out, shape, dev, True)
-    _launch_on(dev, _lib.load().merv_paged_cache_read, "merv_paged_cache_read", cache, *ko, *vo, off_p, start_p, int(total))
+    _launch_on(dev, _lib.load().merv_paged_cache_read, what, cache, *ko, *vo, off_p, start_p, total)
     return k_out, v_out
 
 
@@ -278,22 +297,22 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     natural logarithm of the softmax's sum). A row of length 0 gives zeros and -inf; a length over the table's capacity or a bad page gives
     that row NaN. Sums, softmax and the weights of the values are held in fp32 (the weights as two bf16 numbers); rounded to bf16 once, at the end."""
     what = "paged_decode_attention"
-    cache = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
-    dev = k_pages.device
-    if q.dim() != 3 or q.shape[0] != cache.rows or q.shape[2] != cache.head_dim or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"{what}: q: expected [{cache.rows}, heads, {cache.head_dim}] with heads a multiple of {cache.kv_heads}, got {tuple(q.shape)}")
+    cache, dev, rows, kv_heads, hd, capacity = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
+    qshape = q.shape
+    heads = qshape[1] if len(qshape) == 3 else 0
+    if heads == 0 or qshape[0] != rows or qshape[2] != hd or heads % kv_heads:
+        raise ValueError(f"{what}: q: expected [{rows}, heads, {hd}] with heads a multiple of {kv_heads}, got {tuple(qshape)}")
     if window < 0:
         raise ValueError(f"{what}: window must not be negative")
-    heads = q.shape[1]
-    qr, lens_p = _paged_rows(what, "q", q, q.shape, dev), _paged_ints(what, "lens", lens, cache.rows, dev)
+    qr, lens_p = _paged_rows(what, "q", q, qshape, dev), _paged_ints(what, "lens", lens, rows, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    orow = _paged_rows(what, "out", out, q.shape, dev, True)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+        out = q.new_empty(qshape)
+    orow = _paged_rows(what, "out", out, qshape, dev, True)
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
     lib = _lib.load()
     # a workspace of its own for each call (and each captured graph): nothing is shared by calls that run at the same time
-    nbytes = lib.merv_paged_decode_attention_workspace_bytes(cache.rows, heads, cache.kv_heads, cache.head_dim, cache.table_width * cache.page_size)
+    nbytes = lib.merv_paged_decode_attention_workspace_bytes(rows, heads, kv_heads, hd, capacity)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch_on(dev, lib.merv_paged_decode_attention, what, cache, *qr, *orow, ptr(lse), lens_p, heads, int(window),
-               cache.head_dim**-0.5 if scale is None else float(scale), ptr(ws), nbytes)
+    _launch_on(dev, lib.merv_paged_decode_attention, what, cache, *qr, *orow, 0 if lse is None else lse.data_ptr(), lens_p, heads, int(window),
+               hd**-0.5 if scale is None else float(scale), 0 if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out

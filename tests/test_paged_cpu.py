@@ -77,58 +77,72 @@ def test_tensors_on_the_cpu_are_refused():
         ops.paged_decode_attention(q, pages, pages, table, n)
 
 
+def test_the_packed_structure_is_the_c_one():
+    from merv_amd import _lib, ops
+    values = [(i + 1) * 16 for i in range(len(_lib.PagedCache._fields_))]
+    assert ops._PAGED_CACHE.size == C.sizeof(_lib.PagedCache)
+    c = _lib.PagedCache.from_buffer_copy(ops._PAGED_CACHE.pack(*values))
+    assert [getattr(c, n) for n, _ in _lib.PagedCache._fields_] == values
+
+
 PLAN = r"""
 #include <vector>
 #include "paged_split.h"
 using namespace merv;
 // 0: every unit of every row's pairs is done once, by a worker that has it in the segment it is said to, into a slot of its own, and the join
 // of a pair reads just the slots that were written for it; else a number that names what is wrong
-extern "C" int walk(const int* lens, int rows, int pairs, long window, long capacity, int most, int* used) {
-    long total = 0;
-    std::vector<long> first(rows + 1);
+extern "C" int walk(const int* lens, int rows, int pairs, int window, int capacity, int most, int* used) {
+    int total = 0;
+    std::vector<int> first(rows + 1);
     for (int r = 0; r < rows; ++r) {
         const PagedSpan s = paged_span(lens[r], window, capacity);
         if (lens[r] > 0 && lens[r] <= capacity) {
             if (s.units < 1 || s.base % 16 || s.base > s.lo || s.lo - s.base > 15) return 1;
-            if (s.base + (long)s.units * PAGED_UNIT < s.len || s.base + (long)(s.units - 1) * PAGED_UNIT >= s.len) return 2;
+            if (s.base + s.units * PAGED_UNIT < s.len || s.base + (s.units - 1) * PAGED_UNIT >= s.len) return 2;
             if (s.len - s.lo != (window > 0 && window < lens[r] ? window : lens[r])) return 3;
         } else if (s.units) return 4;
         first[r] = total;
-        total += (long)s.units * pairs;
+        total += s.units * pairs;
     }
     first[rows] = total;
-    const int W = paged_workers(total, most);
-    *used = W;
-    std::vector<int> done(total), slot_of(total, -1), taken(2 * (most > 0 ? most : 1));
+    const PagedShare sh = paged_share(total, most);
+    const int W = *used = sh.workers;
+    if (W > 0 && paged_start(sh, W) != total) return 5;
+    std::vector<int> done(total), slot_of(total, -1), taken(2 * (most > 0 ? most : 1)), last_of(most > 0 ? most : 1, -1), open_slot(most > 0 ? most : 1, -1);
     for (int w = 0; w < W; ++w) {
-        const long a = paged_start(w, total, W), b = paged_start(w + 1, total, W);
-        if (b - a < total / W || b - a > total / W + 1 || b <= a) return 5;
-        for (long x = a; x < b;) {
-            if (paged_owner(x, total, W) != w || paged_owner(b - 1, total, W) != w) return 6;
+        const int a = paged_start(sh, w), b = paged_start(sh, w + 1);
+        if (b - a < total / W || b - a > total / W + 1 || b <= a) return 6;
+        for (int x = a; x < b;) {
+            if (paged_owner(sh, x) != w || paged_owner(sh, b - 1) != w) return 7;
             int r = 0;
             while (first[r + 1] <= x) ++r;
-            const int n = paged_span(lens[r], window, capacity).units, u = (int)((x - first[r]) % n);
-            const long m = n - u < b - x ? n - u : b - x;
-            const int slot = m == n ? -1 : x == a ? 2 * w : 2 * w + 1;
-            if (slot >= 0 && taken[slot]++) return 7;
-            for (long y = x; y < x + m; ++y) done[y]++, slot_of[y] = slot;
+            const int n = paged_span(lens[r], window, capacity).units, u = (x - first[r]) % n;
+            const int m = n - u < b - x ? n - u : b - x;
+            const int slot = m == n ? -1 : paged_slot(w, x == a);
+            if (slot >= 0 && taken[slot]++) return 8;
+            if (u == 0 && m < n) {  // the pair goes on in later workers: one such pair at most
+                if (last_of[w] >= 0) return 9;
+                last_of[w] = paged_owner(sh, x + n - 1);
+                open_slot[w] = slot;
+            }
+            for (int y = x; y < x + m; ++y) done[y]++, slot_of[y] = slot;
             x += m;
         }
     }
-    for (long x = 0; x < total; ++x) if (done[x] != 1) return 8;
-    for (int r = 0; r < rows; ++r) {
-        const int n = paged_span(lens[r], window, capacity).units;
-        for (int p = 0; n && p < pairs; ++p) {
-            const long f = first[r] + (long)p * n;
-            const int w0 = paged_owner(f, total, W), w1 = paged_owner(f + n - 1, total, W);
-            if (w0 == w1) { if (slot_of[f] != -1 || slot_of[f + n - 1] != -1) return 9; continue; }
-            for (int w = w0; w <= w1; ++w) {
-                const long at = paged_start(w, total, W) > f ? paged_start(w, total, W) : f;
-                if (at >= f + n || slot_of[at] != paged_slot(w, f, total, W)) return 10;
-            }
+    for (int x = 0; x < total; ++x) if (done[x] != 1) return 10;
+    int joined = 0, parts = 0;
+    for (int w = 0; w < W; ++w) {
+        if (last_of[w] < 0) continue;
+        if (last_of[w] <= w || last_of[w] >= W) return 11;
+        for (int v = w; v <= last_of[w]; ++v) {
+            const int slot = v == w ? open_slot[w] : 2 * v;
+            if (slot < 0 || taken[slot] != 1) return 12;
+            taken[slot] = 2;  // read, once
+            ++joined;
         }
     }
-    return 0;
+    for (int t : taken) parts += t != 0;
+    return parts == joined ? 0 : 13;
 }
 """
 
@@ -142,7 +156,7 @@ def walk(tmp_path_factory):
     csrc = Path(__file__).resolve().parent.parent / "merv_amd" / "csrc"
     subprocess.check_call(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", f"-I{csrc}", "-o", str(d / "plan.so"), str(d / "plan.cpp")])
     fn = C.CDLL(str(d / "plan.so")).walk
-    fn.argtypes = [C.POINTER(C.c_int), C.c_int, C.c_int, C.c_long, C.c_long, C.c_int, C.POINTER(C.c_int)]
+    fn.argtypes = [C.POINTER(C.c_int)] + [C.c_int] * 5 + [C.POINTER(C.c_int)]
     return fn
 
 

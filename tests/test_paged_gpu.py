@@ -274,6 +274,29 @@ def test_attention_rows_that_fill_the_card(dev):
     check_attention(dev, [150 + 13 * (i % 17) for i in range(70)], 16, 16, 64, 32, "e4m3")
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_attention_short_rows_in_a_large_table(dev, fmt):
+    """The table's capacity, which the launch goes by, is far over the lengths, which the kernel goes by: 140 and 520 pairs left whole by the split kernel, 60 and
+    4100 pairs of a few units shared out by it."""
+    check_attention(dev, [0, 1, 700] + [100 + 9 * i for i in range(32)], 4, 4, 64, 64, fmt, width=100)
+    check_attention(dev, [40 + 5 * i for i in range(65)], 8, 8, 64, 64, fmt, width=100)
+    check_attention(dev, [513, 129, 0, 1024] * 5, 3, 3, 64, 64, fmt, width=100)
+    check_attention(dev, [5, 130] * 21, 100, 100, 64, 64, fmt, width=70)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_attention_pages_of_sixteen_in_unsplit_rows(dev, fmt):
+    """Rows of up to 2048 positions, a workgroup for each pair, with more pages than a wave has lanes."""
+    check_attention(dev, [2048, 0, 1500] + [33 * i for i in range(1, 30)], 8, 4, 64, 16, fmt)
+
+
+def test_attention_joins_of_many_parts(dev):
+    """One row over all workers: more than 16 partial sums to join, one pair (16 heads) and three; and rows that change within a worker."""
+    check_attention(dev, [9000], 16, 1, 64, 32, "bf16")
+    check_attention(dev, [5000, 3], 3, 3, 64, 16, "e4m3")
+    check_attention(dev, [4000 + 100 * i for i in range(14)], 5, 5, 64, 256, "bf16")
+
+
 def test_attention_peaked_and_flat(dev):
     """Scores of some hundreds, where all weight is on one position, and a scale of zero, where all weigh the same."""
     check_attention(dev, [700, 40], 4, 2, 128, 32, "bf16", q_gain=30.0)
