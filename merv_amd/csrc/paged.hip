@@ -103,99 +103,92 @@ MERV_DEVICE void e4m3_unpack8(const u32x2 r, float* f) {
 }
 
 // ---- write ----
-// All vectors of the call (a token's keys, values and queries, token after token) are one line; a block takes WRITE_EACH x 256 / (hd / 16) of them, so it is full
-// whatever the numbers of heads are. A lane holds elements d .. d + 7 of a vector and their partners d + hd/2 .. (the rotation mixes just these), so
-// hd / 16 lanes hold a vector and queries and keys may be rotated in place. The vectors are requested before their places are looked up: the two chains of loads
-// overlap. rot(x) = x cos + rotate_half(x) sin: with bf16 operands and bf16 tables both products are exact in fp32, so the sum's rounding to
-// fp32 and its rounding to bf16 are the only two.
-template <int HD, bool E4M3, int WRITE_EACH>
+// All vectors of the call (a token's keys, values and queries, token after token) are one line, of which a block takes 256 / (hd / 16): it is full whatever the
+// numbers of heads are. A lane holds elements d .. d + 7 of a vector and their partners d + hd/2 .. (the rotation mixes just these), so hd / 16 lanes
+// hold a vector, and queries and keys may be rotated in place. The vectors are requested before their places are looked up: the two chains of loads overlap.
+// rot(x) = x cos + rotate_half(x) sin: with bf16 operands and bf16 tables both products are exact in fp32, so the sum's rounding to fp32 and its
+// rounding to bf16 are the only two.
+// Bound by HBM: 16 prompts of up to 2049 tokens (32 / 8 heads, e4m3, 446 MB moved) 91.8 us, 4.86 TB/s; a prompt of 1049 (28 / 4, bf16) 6.2 us; one token
+// 3.4 us, a chain of three round trips. Stores are non-temporal: 97.7 and 7.4 us without (what reads the queries next does not get slower); two
+// vectors a group of lanes: 92.0 and 7.1 us, and 4.4 for one token.
+template <int HD, bool E4M3>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
     constexpr int LPV = HD / 16, VPB = 256 / LPV;  // lanes for a vector, vectors a block holds at a time
     const int Hkv = p.c.kv_heads, nvec = 2 * Hkv + p.H;
-    const long v0 = (long)blockIdx.x * (VPB * WRITE_EACH), t0 = v0 / nvec;
-    const int r0 = (int)(v0 - t0 * nvec), sub = threadIdx.x % LPV, d0 = sub * 8;
-    long t[WRITE_EACH];
-    int vec[WRITE_EACH];
-    u32x4 raw[WRITE_EACH][2];
-#pragma unroll
-    for (int e = 0; e < WRITE_EACH; ++e) {
-        const unsigned x = r0 + e * VPB + threadIdx.x / LPV;
-        t[e] = t0 + x / (unsigned)nvec;
-        const int i = vec[e] = x % (unsigned)nvec;
-        const bf16_t* src = i >= 2 * Hkv ? p.q + t[e] * p.q_st + (long)(i - 2 * Hkv) * p.q_sh
-                            : i < Hkv    ? p.k + t[e] * p.k_st + (long)i * p.k_sh
-                                         : p.v + t[e] * p.v_st + (long)(i - Hkv) * p.v_sh;
-        if (t[e] < p.T) {
-            raw[e][0] = *(const u32x4*)(src + d0);
-            raw[e][1] = *(const u32x4*)(src + d0 + HD / 2);
-        }
+    const long v0 = (long)blockIdx.x * VPB, t0 = v0 / nvec;
+    const int sub = threadIdx.x % LPV, d0 = sub * 8;
+    const unsigned y = (unsigned)(v0 - t0 * nvec) + threadIdx.x / LPV;
+    const long t = t0 + y / (unsigned)nvec;
+    const int i = y % (unsigned)nvec;
+    const bool is_k = i < Hkv, is_q = i >= 2 * Hkv;
+    const int h = is_q ? i - 2 * Hkv : is_k ? i : i - Hkv;
+    u32x4 olo = {0, 0, 0, 0}, ohi = olo;
+    if (t < p.T) {
+        const bf16_t* src = is_q ? p.q + t * p.q_st + (long)h * p.q_sh : is_k ? p.k + t * p.k_st + (long)h * p.k_sh : p.v + t * p.v_st + (long)h * p.v_sh;
+        olo = *(const u32x4*)(src + d0);
+        ohi = *(const u32x4*)(src + d0 + HD / 2);
     }
     const int row0 = p.offsets ? row_of_token(p.offsets, p.c.rows, t0) : 0;
+    if (t >= p.T) return;
+    const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t, p.offsets ? row_from(p.offsets, p.c.rows, row0, t) : (int)t);
+    if (at.idle) return;
+    const long slot = at.pos & ((1 << p.c.page_log2) - 1);
+    if (p.cos && (is_k || is_q)) {
+        float lo[8], hi[8], cl[8], ch[8], sl[8], sh[8];
+        unpack8f(olo, lo);
+        unpack8f(ohi, hi);
+        const bool in_tables = at.pos < p.rope_len, ok = in_tables && at.page >= 0;
+        const long row = in_tables ? at.pos : 0;
+        unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0), cl);
+        unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0 + HD / 2), ch);
+        unpack8f(*(const u32x4*)(p.sin + row * p.rope_st + d0), sl);
+        unpack8f(*(const u32x4*)(p.sin + row * p.rope_st + d0 + HD / 2), sh);
 #pragma unroll
-    for (int e = 0; e < WRITE_EACH; ++e) {
-        if (t[e] >= p.T) break;
-        const TokenPlace at = place_of_token(p.c, p.offsets, p.start, t[e], p.offsets ? row_from(p.offsets, p.c.rows, row0, t[e]) : (int)t[e]);
-        if (at.idle) continue;
-        const int i = vec[e];
-        const bool is_k = i < Hkv, is_q = i >= 2 * Hkv;
-        const int h = is_q ? i - 2 * Hkv : is_k ? i : i - Hkv;
-        const long slot = at.pos & ((1 << p.c.page_log2) - 1);
-        u32x4 olo = raw[e][0], ohi = raw[e][1];
-        if (p.cos && (is_k || is_q)) {
-            float lo[8], hi[8], cl[8], ch[8], sl[8], sh[8];
-            unpack8f(olo, lo);
-            unpack8f(ohi, hi);
-            const bool in_tables = at.pos < p.rope_len, ok = in_tables && at.page >= 0;
-            const long row = in_tables ? at.pos : 0;
-            unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0), cl);
-            unpack8f(*(const u32x4*)(p.cos + row * p.rope_st + d0 + HD / 2), ch);
-            unpack8f(*(const u32x4*)(p.sin + row * p.rope_st + d0), sl);
-            unpack8f(*(const u32x4*)(p.sin + row * p.rope_st + d0 + HD / 2), sh);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = lo[j], b = hi[j];
-                lo[j] = ok ? a * cl[j] - b * sl[j] : __builtin_nanf("");
-                hi[j] = ok ? b * ch[j] + a * sh[j] : __builtin_nanf("");
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                olo[j] = pack2bf(lo[2 * j], lo[2 * j + 1]);
-                ohi[j] = pack2bf(hi[2 * j], hi[2 * j + 1]);
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float a = lo[j], b = hi[j];
+            lo[j] = ok ? a * cl[j] - b * sl[j] : __builtin_nanf("");
+            hi[j] = ok ? b * ch[j] + a * sh[j] : __builtin_nanf("");
         }
-        if (is_q || (is_k && p.k_out)) {
-            bf16_t* dst = is_q ? p.q_out + t[e] * p.qo_st + (long)h * p.qo_sh : p.k_out + t[e] * p.ko_st + (long)h * p.ko_sh;
-            *(u32x4*)(dst + d0) = olo;
-            *(u32x4*)(dst + d0 + HD / 2) = ohi;
-        }
-        if (is_q) continue;
-        if constexpr (E4M3) {
-            float lo[8], hi[8];
-            unpack8f(olo, lo);  // the cache's numbers are bf16 ones, whichever way it holds them
-            unpack8f(ohi, hi);
-            float amax = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(finite_abs(lo[j]), finite_abs(hi[j])));
-#pragma unroll
-            for (int o = LPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-            const int ex = row_exponent(amax);
-            const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
-            if (at.page < 0) continue;
-            uint8_t* dst = (uint8_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
-            *(u32x2*)(dst + d0) = u32x2{e4m3_pack4(lo, inv), e4m3_pack4(lo + 4, inv)};
-            *(u32x2*)(dst + d0 + HD / 2) = u32x2{e4m3_pack4(hi, inv), e4m3_pack4(hi + 4, inv)};
-            if (sub == 0) (is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] = (uint8_t)(ex + 127);
-        } else {
-            if (at.page < 0) continue;
-            bf16_t* dst = (bf16_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
-            *(u32x4*)(dst + d0) = olo;
-            *(u32x4*)(dst + d0 + HD / 2) = ohi;
+        for (int j = 0; j < 4; ++j) {
+            olo[j] = pack2bf(lo[2 * j], lo[2 * j + 1]);
+            ohi[j] = pack2bf(hi[2 * j], hi[2 * j + 1]);
         }
+    }
+    if (is_q || (is_k && p.k_out)) {
+        bf16_t* dst = is_q ? p.q_out + t * p.qo_st + (long)h * p.qo_sh : p.k_out + t * p.ko_st + (long)h * p.ko_sh;
+        __builtin_nontemporal_store(olo, (u32x4*)(dst + d0));
+        __builtin_nontemporal_store(ohi, (u32x4*)(dst + d0 + HD / 2));
+    }
+    if (is_q) return;
+    if constexpr (E4M3) {
+        float lo[8], hi[8];
+        unpack8f(olo, lo);  // the cache's numbers are bf16 ones, whichever way it holds them
+        unpack8f(ohi, hi);
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(finite_abs(lo[j]), finite_abs(hi[j])));
+#pragma unroll
+        for (int o = LPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+        const int ex = row_exponent(amax);
+        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
+        if (at.page < 0) return;
+        uint8_t* dst = (uint8_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
+        __builtin_nontemporal_store(u32x2{e4m3_pack4(lo, inv), e4m3_pack4(lo + 4, inv)}, (u32x2*)(dst + d0));
+        __builtin_nontemporal_store(u32x2{e4m3_pack4(hi, inv), e4m3_pack4(hi + 4, inv)}, (u32x2*)(dst + d0 + HD / 2));
+        if (sub == 0) (is_k ? p.c.k_scale : p.c.v_scale)[at.page * p.c.ss_page + (long)h * p.c.ss_head + slot] = (uint8_t)(ex + 127);
+    } else {
+        if (at.page < 0) return;
+        bf16_t* dst = (bf16_t*)(is_k ? p.c.k : p.c.v) + at.page * p.c.s_page + (long)h * p.c.s_head + slot * p.c.s_tok;
+        __builtin_nontemporal_store(olo, (u32x4*)(dst + d0));
+        __builtin_nontemporal_store(ohi, (u32x4*)(dst + d0 + HD / 2));
     }
 }
 
 // ---- read ----
 // The same line of vectors, READ_EACH for each group of lanes: all places first, then all loads, then all stores. A lane moves 16 bytes of the cache.
+// Bound by HBM: 32 rows of up to 4000 positions (2 kv heads, bf16, 154 MB moved) 27.0 us, 5.7 TB/s with two, 29.0 with one, 28.5 with four; 41.4 without
+// non-temporal stores. 1049 positions (8 kv heads, e4m3): 4.0 us with one, 4.8 with two.
 template <int HD, bool E4M3, int READ_EACH>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
     constexpr int LPV = E4M3 ? HD / 16 : HD / 8, VPB = 256 / LPV, EPL = HD / LPV;
@@ -238,10 +231,10 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
             u32x4 o[2];
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j >> 2][j & 3] = pack2bf(ldexpf(f[2 * j], ex[e]), ldexpf(f[2 * j + 1], ex[e]));
-            *(u32x4*)dst[e] = o[0];
-            *(u32x4*)(dst[e] + 8) = o[1];
+            __builtin_nontemporal_store(o[0], (u32x4*)dst[e]);
+            __builtin_nontemporal_store(o[1], (u32x4*)(dst[e] + 8));
         } else {
-            *(u32x4*)dst[e] = x[e];
+            __builtin_nontemporal_store(x[e], (u32x4*)dst[e]);
         }
     }
 }
@@ -850,17 +843,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs p) {
 
 }  // namespace
 
-// EACH vectors for each group of lanes: as many as still leave the card two workgroups a CU or more
-template <int HD, bool E4M3, int EACH>
-static void launch_paged_write_each(const PagedWriteArgs& a, long vectors, hipStream_t s) {
-    const long each = 256 / (HD / 16) * EACH;
-    hipLaunchKernelGGL((paged_write_kernel<HD, E4M3, EACH>), dim3((unsigned)((vectors + each - 1) / each)), dim3(256), 0, s, a);
-}
 template <int HD, bool E4M3>
 static void launch_paged_write_as(const PagedWriteArgs& a, hipStream_t s) {
-    const long vectors = (long)a.T * (2 * a.c.kv_heads + a.H);
-    if (vectors >= 512L * 2 * 256 / (HD / 16)) launch_paged_write_each<HD, E4M3, 2>(a, vectors, s);
-    else launch_paged_write_each<HD, E4M3, 1>(a, vectors, s);
+    const long vectors = (long)a.T * (2 * a.c.kv_heads + a.H), each = 256 / (HD / 16);
+    hipLaunchKernelGGL((paged_write_kernel<HD, E4M3>), dim3((unsigned)((vectors + each - 1) / each)), dim3(256), 0, s, a);
 }
 
 hipError_t launch_paged_write(const PagedWriteArgs& a, hipStream_t s) {
@@ -879,7 +865,8 @@ static void launch_paged_read_each(const PagedReadArgs& a, long vectors, hipStre
 template <int HD, bool E4M3>
 static void launch_paged_read_as(const PagedReadArgs& a, hipStream_t s) {
     const long vectors = (long)a.T * 2 * a.c.kv_heads;
-    if (vectors >= 512L * 4 * 256 / (E4M3 ? HD / 16 : HD / 8)) launch_paged_read_each<HD, E4M3, 4>(a, vectors, s);
+    // two vectors for a group of lanes where that leaves the card two workgroups a CU
+    if (vectors >= 512L * 2 * 256 / (E4M3 ? HD / 16 : HD / 8)) launch_paged_read_each<HD, E4M3, 2>(a, vectors, s);
     else launch_paged_read_each<HD, E4M3, 1>(a, vectors, s);
 }
 

@@ -155,22 +155,22 @@ _PAGED_CACHE = struct.Struct("@5P7q6i")  # merv_paged_cache
 def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written: bool = False):
     """-> (the C structure, device, rows, kv_heads, head_dim, positions that a row's table can hold)."""
     kind, shape, dev = k_pages.dtype, k_pages.shape, k_pages.device
-    if kind not in (torch.bfloat16, torch.float8_e4m3fn) or len(shape) != 4 or dev.type != "cuda":
+    if (kind is not _BF16 and kind is not _E4M3) or len(shape) != 4 or not k_pages.is_cuda:
         raise ValueError(f"{what}: expected CUDA pages [n_pages, kv_heads, page_size, head_dim] of bfloat16 or float8_e4m3fn, got "
                          f"{kind} {tuple(shape)} on {dev}")
     st = k_pages.stride()
-    if v_pages.dtype != kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.device != dev:
+    if v_pages.dtype is not kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.device != dev:
         raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
     n_pages, kv_heads, page, hd = shape
     if st[3] != 1:
         raise ValueError(f"{what}: the pages' last dimension must be contiguous")
-    rows, width = table.shape if table.dim() == 2 else (-1, -1)
     tst = table.stride()
-    if rows < 0 or table.dtype != torch.int32 or table.device != dev or (tst[1] != 1 and width > 1):
+    rows, width = table.shape if len(tst) == 2 else (-1, -1)
+    if rows < 0 or table.dtype is not torch.int32 or table.device != dev or (tst[1] != 1 and width > 1):
         raise ValueError(f"{what}: expected an int32 table [rows, width] on {dev} with contiguous rows")
     ks = vs = 0
     sst = (0, 0)
-    if kind != torch.bfloat16:
+    if kind is _E4M3:
         if k_scales is None or v_scales is None:
             raise ValueError(f"{what}: float8_e4m3fn pages need k_scales and v_scales")
         sst = k_scales.stride()
@@ -188,13 +188,13 @@ def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written
     c = PagedCache.from_buffer_copy(_PAGED_CACHE.pack(
         k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), n_pages, st[0] if n_pages > 1 else 0, st[1] if kv_heads > 1 else 0, st[2],
         sst[0] if n_pages > 1 else 0, sst[1] if kv_heads > 1 else 0, tst[0] if rows > 1 else 0, rows, width, kv_heads, hd, page,
-        KV_BF16 if kind == torch.bfloat16 else KV_E4M3))
+        KV_E4M3 if kind is _E4M3 else KV_BF16))
     return c, dev, rows, kv_heads, hd, width * page
 
 
 def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev, out: bool = False):
     st = t.stride()
-    if t.dtype != torch.bfloat16 or t.shape != shape or t.device != dev or st[2] != 1:
+    if t.dtype is not _BF16 or t.shape != shape or t.device != dev or st[2] != 1:
         raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on {dev} with contiguous last dimension, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     s0, s1 = st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0
@@ -206,18 +206,23 @@ def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev, out: bool = F
 def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != dev or (t.stride(0) != 1 and n > 1):
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.device != dev or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # a hundredth of torch.cuda.current_stream(dev).cuda_stream's 1.9 us
+_E4M3, _BF16 = torch.float8_e4m3fn, torch.bfloat16
+
+
 def _launch_on(dev, call, what: str, *args) -> None:
     """call(*args, stream) on the device's current stream; the device is made current where it is not (its null stream has no device of its own)."""
-    if torch.cuda.current_device() == dev.index:
-        rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
+    i = dev.index
+    if torch._C._cuda_getDevice() == i:
+        rc = call(*args, _raw_stream(i))
     else:
         with torch.cuda.device(dev):
-            rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = call(*args, _raw_stream(i))
     if rc:
         check(rc, what)
 
@@ -257,7 +262,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
         heads = qshape[1]
         qr = _paged_rows(what, "q", q, qshape, dev)
         if q_out is None:
-            q_out = q.new_empty(qshape)
+            q_out = torch.empty_like(q)
         qo = _paged_rows(what, "q_out", q_out, qshape, dev, True)
     elif q_out is not None:
         raise ValueError(f"{what}: q_out needs q")
@@ -306,7 +311,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         raise ValueError(f"{what}: window must not be negative")
     qr, lens_p = _paged_rows(what, "q", q, qshape, dev), _paged_ints(what, "lens", lens, rows, dev)
     if out is None:
-        out = q.new_empty(qshape)
+        out = torch.empty_like(q)
     orow = _paged_rows(what, "out", out, qshape, dev, True)
     lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
     lib = _lib.load()
