@@ -146,7 +146,7 @@ class LlamaBackbone:
                              temperature: float = 1.0, eos_token_id: Optional[int] = None,
                              generator: Optional[torch.Generator] = None, use_graph: bool = True, top_k: int = 0,
                              top_p: Optional[float] = 1.0, repetition_penalty: Optional[float] = 1.0, min_new_tokens: int = 0,
-                             use_hip_decode: bool = True, prompt_ids: Optional[torch.LongTensor] = None) -> torch.LongTensor:
+                             use_hip_decode: bool = True, prompt_ids: Optional[torch.LongTensor] = None, kv_cache: str = "static") -> torch.LongTensor:
         """Prefill on `inputs_embeds` [B, S, D] (merv.py:723-734), then decode token by token on the KV cache
         (merv.py:524-538). Returns the new token ids [B, <= max_new_tokens]. Decoding controls are the subset of HF
         `generate` kwargs the reference's scripts pass through (merv.py:818-825): greedy or sampling with `temperature`,
@@ -154,14 +154,43 @@ class LlamaBackbone:
         top-p). The reference hands `input_ids` to HF generate (merv.py:819), so HF's RepetitionPenaltyLogitsProcessor penalises
         the PROMPT's tokens as well as the generated ones: pass them as `prompt_ids` [B, S_text] (MERV.generate does) to get the
         same set; without them only generated tokens are penalised. `None` for top_p / repetition_penalty / top_k means "off",
-        as in HF's GenerationConfig."""
+        as in HF's GenerationConfig.
+
+        kv_cache "paged" / "paged-e4m3": a paged cache in bf16 / 8 bits (merv_amd.paged.PagedDecoder). `inputs_embeds` may then be a list of [S_b, D], prompts
+        of lengths of their own (and `prompt_ids` a list of 1-D tensors); all rows are decoded together. Up to the 8-bit rounding the tokens are those that
+        each prompt alone would get, behind a row's end of sequence they mean nothing."""
+        if kv_cache not in ("static", "paged", "paged-e4m3"):
+            raise ValueError(f"unknown kv_cache `{kv_cache}` (static, paged or paged-e4m3)")
+        if kv_cache == "static" and not torch.is_tensor(inputs_embeds):
+            raise ValueError("prompts of several lengths need kv_cache='paged' or 'paged-e4m3'")
+        rows, dev = len(inputs_embeds), inputs_embeds[0].device
+        if isinstance(prompt_ids, (list, tuple)):  # of several lengths: padded with a row's own first id (the penalty counts an id once)
+            most = max(p.numel() for p in prompt_ids)
+            prompt_ids = torch.stack([torch.cat([p.reshape(-1), p.reshape(-1)[:1].expand(most - p.numel())]) for p in prompt_ids])
         top_p = 1.0 if top_p is None else float(top_p)
         repetition_penalty = 1.0 if repetition_penalty is None else float(repetition_penalty)
         top_k = int(top_k or 0)
         dec = None
-        if use_graph and self._needs_hf_decode(inputs_embeds.shape[1] + max_new_tokens + 1):
+        if kv_cache != "static":
+            from .paged import PagedDecoder
+            need = max(e.shape[0] for e in inputs_embeds) + max_new_tokens + 1
+            if need > self.config.max_position_embeddings:
+                raise ValueError(f"{need} positions are needed, the model has {self.config.max_position_embeddings}")
+            bucket = min((need + 255) // 256 * 256, self.config.max_position_embeddings)
+            key = (bucket, rows, kv_cache)
+            if not hasattr(self, "_decoders"):
+                self._decoders = {}
+            if key not in self._decoders:
+                self._decoders.clear()
+                self._decoders[key] = PagedDecoder(self.llm, bucket, rows, fmt="e4m3" if kv_cache == "paged-e4m3" else "bf16")
+            dec = self._decoders[key]
+            logits = dec.prefill(inputs_embeds, room=max_new_tokens + 1)
+            step = lambda tok: dec.decode(tok, use_graph=use_graph)
+        elif use_graph and self._needs_hf_decode(inputs_embeds.shape[1] + max_new_tokens + 1):
             use_graph = False  # the static-cache decoders implement neither sliding-window attention nor MLP biases
-        if use_graph and inputs_embeds.is_cuda and inputs_embeds.shape[1] + max_new_tokens + 1 <= self.config.max_position_embeddings:
+        if dec is not None:
+            pass
+        elif use_graph and inputs_embeds.is_cuda and inputs_embeds.shape[1] + max_new_tokens + 1 <= self.config.max_position_embeddings:
             # static-cache prefill + hipGraph-replayed decode steps (StaticDecoder above)
             need = inputs_embeds.shape[1] + max_new_tokens + 1
             bucket = min((need + 255) // 256 * 256, self.config.max_position_embeddings)  # cache length, reused across calls
@@ -217,7 +246,7 @@ class LlamaBackbone:
                     ids = ids[:, : int(hit[0]) + 1]
             return ids
         new_tokens = []
-        done = torch.zeros(inputs_embeds.shape[0], dtype=torch.bool, device=inputs_embeds.device)
+        done = torch.zeros(rows, dtype=torch.bool, device=dev)
         for i in range(max_new_tokens):
             if eos_token_id is not None and i < min_new_tokens:  # HF MinLength / MinNewTokensLength processors
                 logits = logits.clone()
@@ -290,14 +319,17 @@ class StaticDecoder:
             fr = torch.outer(torch.arange(max_len, dtype=torch.float32, device=self.dev), inv)
             emb = torch.cat([fr, fr], dim=-1)
             self.cos, self.sin = emb.cos().to(self.dt), emb.sin().to(self.dt)  # [max_len, hd]
-        L = cfg.num_hidden_layers
-        self.K = [torch.zeros(batch, self.Hkv, max_len, self.hd, dtype=self.dt, device=self.dev) for _ in range(L)]
-        self.V = [torch.zeros(batch, self.Hkv, max_len, self.hd, dtype=self.dt, device=self.dev) for _ in range(L)]
+        self._allocate()
         self.ar = torch.arange(max_len, device=self.dev)
         # the token a step embeds: ONE tensor for the decoder's life. Every captured graph (decode(), HipDecoder.greedy_run) reads and
         # writes THIS storage; callers only ever copy_ into it (rebinding it after a capture would leave that graph on freed memory).
         self.tok = torch.zeros(batch, 1, dtype=torch.long, device=self.dev)
         self.graph = None
+
+    def _allocate(self) -> None:
+        L, batch, max_len = self.cfg.num_hidden_layers, self.B, self.max_len
+        self.K = [torch.zeros(batch, self.Hkv, max_len, self.hd, dtype=self.dt, device=self.dev) for _ in range(L)]
+        self.V = [torch.zeros(batch, self.Hkv, max_len, self.hd, dtype=self.dt, device=self.dev) for _ in range(L)]
 
     def _rms(self, x, w):
         xf = x.float()

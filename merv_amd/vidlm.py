@@ -234,7 +234,7 @@ class MERV(MERVVisual):
         max_new = kwargs.pop("max_new_tokens", 32)
         gen = dict(max_new_tokens=max_new, do_sample=kwargs.pop("do_sample", False), temperature=kwargs.pop("temperature", 1.0),
                    top_k=kwargs.pop("top_k", 0) or 0, top_p=kwargs.pop("top_p", 1.0) or 1.0,
-                   repetition_penalty=kwargs.pop("repetition_penalty", 1.0) or 1.0)
+                   repetition_penalty=kwargs.pop("repetition_penalty", 1.0) or 1.0, kv_cache=kwargs.pop("kv_cache", "static"))
         # HF generate kwargs the reference forwards (merv.py:818-825) that change nothing here, or that this explicit
         # prefill + decode loop does not implement: the former are accepted, the latter fail loudly instead of silently
         # decoding differently from the reference's eval scripts

@@ -174,3 +174,25 @@ def test_the_work_is_shared_out_whole(walk):
         rc = walk((C.c_int * len(lens))(*lens), len(lens), pairs, window, capacity, most, C.byref(used))
         assert rc == 0, (rc, lens, pairs, window, capacity, most)
         assert 0 <= used.value <= most
+
+
+def test_pages_are_handed_out_once():
+    from merv_amd.paged import PagedKVCache
+    c = PagedKVCache(2, 3, 100, 2, 64, "cpu", "e4m3", page_size=16, n_pages=12)
+    table = c.table
+    c.assign([100, 0, 17])
+    assert c.table is table and table.shape == (3, 7)
+    used = table[table >= 0].tolist()
+    assert len(used) == len(set(used)) == 9 and max(used) < 12
+    assert (table[1] == -1).all() and (table[2, :2] >= 0).all() and (table[2, 2:] == -1).all()
+    lay = c.layer(1)
+    assert lay["k_pages"].shape == (12, 2, 16, 64) and lay["k_scales"].shape == (12, 2, 16) and lay["table"] is table
+    c.assign([0, 16, 0])
+    assert (c.table >= 0).sum() == 1
+    for bad, msg in (([100, 100, 100], "pages needed"), ([101, 0, 0], "at most"), ([1, 1], "3 rows"), ([-1, 0, 0], "at most")):
+        with pytest.raises(ValueError, match=msg):
+            c.assign(bad)
+    with pytest.raises(ValueError, match="format"):
+        PagedKVCache(1, 1, 16, 1, 64, "cpu", "fp4")
+    with pytest.raises(ValueError, match="page_size"):
+        PagedKVCache(1, 1, 16, 1, 64, "cpu", page_size=24)
