@@ -245,7 +245,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
 //                4 (lane / 16) + i of each half tile -- which is, half after half, the layout of the B operand of
 //   O^T += V^T P^T (A = 16 dims x 32 positions): the order of the summed positions is free, so P goes from one product into the other in registers.
 // V's operand wants 8 positions of one dim in a lane; a lane loads 8 positions x HD/16 neighbouring dims in whole lines and transposes them in registers
-// (v_perm_b32), row r of product dt being dim r * HD/16 + dt. Nothing passes through LDS until the four waves of a workgroup meet.
+// (v_perm_b32), row r of product dt being dim r * HD/16 + dt. K's operand wants a key in a lane: loaded so, a wave's 64 16-byte pieces lie in 16 lines of memory
+// (62 GB/s a CU); loaded in whole lines and turned in the wave's own corner of LDS, 80 (16 bits; one row of 4096 positions, unsplit, 38.6 and 30.2 us).
 // Scores, maximum, sum and output are fp32. A weight p is used as the sum of two bf16 numbers, p cut off and the rest rounded (2^-15 relative: one bf16
 // alone would add as much error as the output's own rounding); where values may be infinite the rest is kept above zero (by 2^-20 p), so that it
 // neither turns an infinity round nor makes it NaN. The running maximum moves only when a score exceeds it by 2^6: the rescaling of the 32 output
@@ -255,10 +256,10 @@ constexpr float RAISE = 6.f;
 
 template <int HD, bool E4M3>
 struct PagedTile {  // 32 positions of one head in a wave's registers
-    static constexpr int DV = HD / 16;                  // dims of a value in a lane
-    static constexpr int KL = E4M3 ? HD / 64 : HD / 32; // 16-byte loads of a key's lane share
-    static constexpr int VW = E4M3 ? DV / 4 : DV / 2;   // words of a value's lane share
-    u32x4 k[2][KL];
+    static constexpr int DV = HD / 16;                   // dims of a value in a lane
+    static constexpr int CPR = HD * (E4M3 ? 1 : 2) / 16; // 16-byte chunks of a key
+    static constexpr int VW = E4M3 ? DV / 4 : DV / 2;    // words of a value's lane share
+    u32x4 k[CPR / 2];
     uint32_t v[8][VW];
     uint32_t ks[2], vs[2];
 };
@@ -311,9 +312,9 @@ MERV_DEVICE void load_tile(PagedTile<HD, E4M3>& t, const PagedCacheArgs& c, cons
         const long off = (id * c.s_page + (long)at.hkv * c.s_head + slot * c.s_tok) * ELT;
         const char* kp = (const char*)c.k + off;
         const char* vp = (const char*)c.v + off;
-        const unsigned krow = (unsigned)r * (unsigned)(c.s_tok * ELT) + tg * 16;
+        const unsigned krow = (unsigned)(lane / Tile::CPR) * (unsigned)(c.s_tok * ELT) + lane % Tile::CPR * 16;
 #pragma unroll
-        for (int j = 0; j < Tile::KL; ++j) t.k[tt][j] = *(const u32x4*)(kp + (krow + j * 64));
+        for (int i = 0; i < Tile::CPR / 4; ++i) t.k[tt * (Tile::CPR / 4) + i] = *(const u32x4*)(kp + i * (64 / Tile::CPR) * c.s_tok * ELT + krow);
         const unsigned vrow = (unsigned)tg * 4u * (unsigned)(c.s_tok * ELT) + r * Tile::DV * ELT;
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words(t.v[tt * 4 + i], vp + i * c.s_tok * ELT + vrow);
@@ -332,21 +333,35 @@ struct PagedState {  // of a wave: lane l has head l % 16
 };
 
 template <int HD, bool E4M3>
-MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int tok, int lo, int len) {
+MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int tok, int lo, int len, char* room) {
     typedef PagedTile<HD, E4M3> Tile;
+    constexpr int CPR = Tile::CPR, RPL = 16 / CPR;  // keys in 256 bytes of LDS
     const int lane = threadIdx.x & 63, tg = lane >> 4;
+    // keys pass through the wave's own part of LDS: loaded in whole lines, 64 / CPR at a time, wanted a key in a lane. Chunk c of key j lies at c ^ (j / RPL): the
+    // 16 lanes of one access, here and below, touch all banks once.
+#pragma unroll
+    for (int i = 0; i < CPR / 2; ++i) {
+        const int j = i * (64 / CPR) + lane / CPR;
+        *(u32x4*)(room + j * (CPR * 16) + ((lane % CPR) ^ (j / RPL % CPR)) * 16) = t.k[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     f32x4 s[2];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
         s[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        u32x4 codes = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
+            const int key = tt * 16 + (lane & 15);
+            auto chunk = [&](int c) { return *(const u32x4*)(room + key * (CPR * 16) + (c ^ (key / RPL % CPR)) * 16); };
             bf16x8 a;
             if constexpr (E4M3) {
-                const uint32_t w0 = t.k[tt][j >> 1][(j & 1) * 2], w1 = t.k[tt][j >> 1][(j & 1) * 2 + 1];
+                if ((j & 1) == 0) codes = chunk((j >> 1) * 4 + tg);
+                const uint32_t w0 = codes[(j & 1) * 2], w1 = codes[(j & 1) * 2 + 1];
                 a = __builtin_bit_cast(bf16x8, u32x4{e4m3_pair(w0, 0), e4m3_pair(w0, 1), e4m3_pair(w1, 0), e4m3_pair(w1, 1)});
             } else {
-                a = __builtin_bit_cast(bf16x8, t.k[tt][j]);
+                a = __builtin_bit_cast(bf16x8, chunk(j * 4 + tg));
             }
             s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[j], s[tt], 0, 0, 0);
         }
@@ -449,47 +464,51 @@ MERV_DEVICE PagedSpan span_of(const PagedAttnArgs& p, int row) {
     return span_of_len(p, *(const __attribute__((address_space(4))) int*)(uintptr_t)(p.lens + row));
 }
 
-// The workspace: a PagedOpen of each worker, then two partial sums (PAGED_HEAD_BLOCK heads of HD numbers, maximum, sum, 2 of padding) of each.
+// The workspace: a PagedOpen of each worker, then two partial sums of each (of a head: HD numbers, maximum, sum, 2 of padding).
 struct PagedOpen {  // of the pair that begins in a worker and ends in a later one
     int row, pair, slot, last;  // last: the worker that it ends in, -1: there is no such pair
 };
+// (the first sums of all workers, then the second ones: those of one pair, most of them first ones, lie together)
 template <int HD>
-MERV_DEVICE float* paged_sums(const PagedAttnArgs& p) {
-    return (float*)((PagedOpen*)p.ws + p.workers);
+MERV_DEVICE float* paged_sum(const PagedAttnArgs& p, int slot, int head) {
+    const int block = min(p.H / p.c.kv_heads, PAGED_HEAD_BLOCK);
+    return (float*)((PagedOpen*)p.ws + p.workers) + ((size_t)((slot & 1) * p.workers + (slot >> 1)) * block + head) * (HD + 4);
 }
 
-template <int HD>
+template <int HD, int NW>
 struct PagedLds {
-    float o[4][PAGED_HEAD_BLOCK][HD + 4];  // (padded: heads lie in other banks)
-    float m[4][PAGED_HEAD_BLOCK], l[4][PAGED_HEAD_BLOCK];
+    float o[NW][PAGED_HEAD_BLOCK][HD + 4];  // (padded: heads lie in other banks)
+    float m[NW][PAGED_HEAD_BLOCK], l[NW][PAGED_HEAD_BLOCK];
 };
 
 struct PagedSegment {  // units u .. u + n - 1 of one pair. slot < 0: all of the pair, the result is written.
     int base, lo, len, units, row, pair, u, n, slot;
 };
 
-// What a wave holds of a segment: its tiles are 32 positions at first + 128 i, the pages of 32 of them at a time lie in `ids`, one half tile in each lane.
+// What a wave (of NW) holds of a segment: its tiles are 32 positions at first + 32 NW i, the pages of 32 of them at a time lie in `ids`, one half tile in each lane.
 struct PagedWalk {
     int first, tiles, ids;
 };
 
+template <int NW>
 MERV_DEVICE int half_tile(const PagedSegment& g, int first, int t0) {  // the lane's one of 32 tiles from t0 on
     const int lane = threadIdx.x & 63;
-    return min(first + (t0 + (lane >> 1)) * PAGED_UNIT + (lane & 1) * 16, g.len - 1);  // behind the row's end: the row's last position
+    return min(first + (t0 + (lane >> 1)) * (32 * NW) + (lane & 1) * 16, g.len - 1);  // behind the row's end: the row's last position
 }
+template <int NW>
 MERV_DEVICE int load_ids(const PagedAttnArgs& p, const PagedSegment& g, int first, int t0) {
-    return (p.c.table + (long)g.row * p.c.table_stride)[half_tile(g, first, t0) >> p.c.page_log2];
+    return (p.c.table + (long)g.row * p.c.table_stride)[half_tile<NW>(g, first, t0) >> p.c.page_log2];
 }
 
 // `pages`, where given: the row's pages, one in each lane
-template <bool GIVEN>
+template <int NW, bool GIVEN>
 MERV_DEVICE PagedWalk begin_walk(const PagedAttnArgs& p, const PagedSegment& g, int pages) {
     PagedWalk w;
     w.first = g.base + g.u * PAGED_UNIT + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
     const int left = g.len - w.first;
-    w.tiles = left <= 0 || p.c.n_pages <= 0 ? 0 : min(g.n, (left + PAGED_UNIT - 1) / PAGED_UNIT);
-    if (GIVEN && p.c.table_width <= 64) w.ids = __shfl(pages, half_tile(g, w.first, 0) >> p.c.page_log2, 64);
-    else w.ids = load_ids(p, g, w.first, 0);
+    w.tiles = left <= 0 || p.c.n_pages <= 0 ? 0 : (min(left, g.n * PAGED_UNIT) + 32 * NW - 1) / (32 * NW);
+    if (GIVEN && p.c.table_width <= 64) w.ids = __shfl(pages, half_tile<NW>(g, w.first, 0) >> p.c.page_log2, 64);
+    else w.ids = load_ids<NW>(p, g, w.first, 0);
     return w;
 }
 
@@ -500,8 +519,9 @@ MERV_DEVICE int checked_ids(const PagedAttnArgs& p, int ids, int& bad) {
     return ok ? ids : 0;
 }
 
+template <int NW>
 MERV_DEVICE PagedAt tile_at(const PagedAttnArgs& p, const PagedSegment& g, const PagedWalk& w, int i) {
-    const int tok = w.first + i * PAGED_UNIT, mask = (1 << p.c.page_log2) - 1;
+    const int tok = w.first + i * (32 * NW), mask = (1 << p.c.page_log2) - 1;
     const int half1 = tok + 16 < g.len ? tok + 16 : tok;  // behind the row's end: the first half again
     return PagedAt{g.pair / p.head_blocks, tok & mask, half1 & mask, __builtin_amdgcn_readlane(w.ids, 2 * (i & 31)),
                    __builtin_amdgcn_readlane(w.ids, 2 * (i & 31) + 1)};
@@ -520,9 +540,9 @@ MERV_DEVICE void load_queries(bf16x8 (&q)[HD / 32], const PagedAttnArgs& p, cons
     }
 }
 
-// the four waves' sums of a segment, together: the result, or a partial sum
-template <int HD>
-MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD>& lds, const PagedSegment& g, PagedState<HD>& st, int bad) {
+// the waves' sums of a segment, together: the result, or a partial sum
+template <int HD, int NW>
+MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD, NW>& lds, const PagedSegment& g, PagedState<HD>& st, int bad) {
     constexpr int DV = HD / 16;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
@@ -543,13 +563,16 @@ MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD>& lds, const Pa
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < heads * (HD / 4); e += 256) {
+    for (int e = threadIdx.x; e < heads * (HD / 4); e += 64 * NW) {
         const int hh = e / (HD / 4), d = e % (HD / 4) * 4;
-        const float M = fmaxf(fmaxf(lds.m[0][hh], lds.m[1][hh]), fmaxf(lds.m[2][hh], lds.m[3][hh])), base = M == -INFINITY ? 0.f : M;
+        float M = lds.m[0][hh];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, lds.m[w][hh]);
+        const float base = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(lds.m[w][hh] - base);
             L += f * lds.l[w][hh];
             O += f * *(const f32x4*)&lds.o[w][hh][d];
@@ -559,7 +582,7 @@ MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD>& lds, const Pa
             *(u32x2*)(p.out + (long)g.row * p.o_st + (long)(h0 + hh) * p.o_sh + d) = o;
             if (p.lse && d == 0) p.lse[(long)g.row * p.H + h0 + hh] = (M + __builtin_amdgcn_logf(L)) * LN2;
         } else {
-            float* ws = paged_sums<HD>(p) + ((size_t)g.slot * PAGED_HEAD_BLOCK + hh) * (HD + 4);
+            float* ws = paged_sum<HD>(p, g.slot, hh);
             *(f32x4*)(ws + d) = O;
             if (d == 0) *(f32x2*)(ws + HD) = f32x2{M, L};
         }
@@ -591,14 +614,15 @@ MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
 // the compiler wait, at each use, for the newer loads too. Lengths come through the scalar cache for the same reason.
 //
 // Bound by HBM where the call is large, by its chain of round trips (length, pages, keys and values, sums) where it is small. Measured, 128 dims:
-//   96 rows of 2458 .. 8192 positions, 32 / 8 heads, 16 bits: 354 us, 5.84 TB/s of keys and values (a copy of 1 GiB on this card: 5.05)
-//   1 row of 131072, 32 / 8 heads, 8 bits: 59 us, 4.55 TB/s, 8 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21 us, 2.9 TB/s
-//   1 row of 77, 16 / 2 heads: 4.6 us;  1 row of 1049, 32 / 32, 16 bits: 13.5 us, 3.9 of them the join
+//   96 rows of 2458 .. 8192 positions, 32 / 8 heads, 16 bits: 352 us, 5.87 TB/s of keys and values (a copy of 1 GiB on this card: 5.05)
+//   1 row of 131072, 32 / 8 heads, 8 bits: 60 us, 4.5 TB/s, 8 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21.7 us, 2.8 TB/s
+//   1 row of 77, 16 / 2 heads: 4.5 us;  1 row of 1049, 32 / 32, 16 bits: 11.2 us
 // 512 workers: with 1024 the large call takes 363 us and 33 x 3001 takes a fifth more (twice the segments); with 256 half the loads are on their way.
 // Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit.
-template <int HD, bool E4M3, bool DIRECT>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p) {
-    __shared__ PagedLds<HD> lds;
+template <int HD, bool E4M3, bool DIRECT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnArgs p) {
+    static_assert(DIRECT || NW == 4, "a unit is one tile for each of four waves");
+    __shared__ PagedLds<HD, NW> lds;
     const int pairs = p.c.kv_heads * p.head_blocks;
     PagedSegment g;
     int x = 0, end = 0, w = 0;  // units of the line: behind this segment, behind this worker; the worker
@@ -658,7 +682,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p
         if (sp.units == 0) {
             const int group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
             const int heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
-            for (int e = threadIdx.x; e < heads * HD; e += 256) write_unseen<HD>(p, g.row, hkv * group + hb * PAGED_HEAD_BLOCK + e / HD, e % HD);
+            for (int e = threadIdx.x; e < heads * HD; e += 64 * NW) write_unseen<HD>(p, g.row, hkv * group + hb * PAGED_HEAD_BLOCK + e / HD, e % HD);
             return;
         }
         g.base = sp.base, g.lo = sp.lo, g.len = sp.len, g.units = sp.units;
@@ -667,11 +691,12 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p
     const float scale2 = p.scale * LOG2E;
     PagedTile<HD, E4M3> a, b;
     bf16x8 q[HD / 32];
+    char* room = (char*)&lds.o[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)][0][0];
     int bad = 0;
-    PagedWalk walk = begin_walk<DIRECT>(p, g, pages);
+    PagedWalk walk = begin_walk<NW, DIRECT>(p, g, pages);
     load_queries<HD, E4M3>(q, p, g);
     walk.ids = checked_ids(p, walk.ids, bad);
-    if (walk.tiles > 0) load_tile(a, p.c, tile_at(p, g, walk, 0));
+    if (walk.tiles > 0) load_tile(a, p.c, tile_at<NW>(p, g, walk, 0));
     for (;;) {
         PagedSegment g2 = g;
         PagedWalk walk2 = walk;
@@ -692,7 +717,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p
                 g2.slot = g2.n == g2.units ? -1 : paged_slot(w, false);
                 if (g2.n < g2.units) open = PagedOpen{g2.row, g2.pair, g2.slot, paged_owner(share, x + g2.units - 1)};
                 x += g2.n;
-                walk2 = begin_walk<false>(p, g2, 0);
+                walk2 = begin_walk<NW, false>(p, g2, 0);
             }
         }
         PagedState<HD> st;
@@ -703,34 +728,34 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PagedAttnArgs p
         // where the tile behind i lies
         auto behind = [&](int i) {
             if (i + 1 < walk.tiles) {
-                if (((i + 1) & 31) == 0) walk.ids = checked_ids(p, load_ids(p, g, walk.first, i + 1), bad);
-                return tile_at(p, g, walk, i + 1);
+                if (((i + 1) & 31) == 0) walk.ids = checked_ids(p, load_ids<NW>(p, g, walk.first, i + 1), bad);
+                return tile_at<NW>(p, g, walk, i + 1);
             }
             if (more && walk2.tiles > 0) {
                 walk2.ids = checked_ids(p, walk2.ids, bad2);
-                return tile_at(p, g2, walk2, 0);
+                return tile_at<NW>(p, g2, walk2, 0);
             }
-            return tile_at(p, g, walk, i);
+            return tile_at<NW>(p, g, walk, i);
         };
         bool in_b = false;  // the next segment's first tile
         for (int i = 0; i < walk.tiles;) {
             load_tile(b, p.c, behind(i));
             __builtin_amdgcn_sched_barrier(0);  // all of the next tile is requested before the first wait for this one
-            use_tile(st, a, q, scale2, walk.first + i * PAGED_UNIT, g.lo, g.len);
+            use_tile(st, a, q, scale2, walk.first + i * (32 * NW), g.lo, g.len, room);
             if (++i == walk.tiles) {
                 in_b = true;
                 break;
             }
             load_tile(a, p.c, behind(i));
             __builtin_amdgcn_sched_barrier(0);
-            use_tile(st, b, q, scale2, walk.first + i * PAGED_UNIT, g.lo, g.len);
+            use_tile(st, b, q, scale2, walk.first + i * (32 * NW), g.lo, g.len, room);
             ++i;
         }
         if (more) {
             load_queries<HD, E4M3>(q, p, g2);
             if (walk.tiles == 0 && walk2.tiles > 0) {  // else it is on its way
                 walk2.ids = checked_ids(p, walk2.ids, bad2);
-                load_tile(a, p.c, tile_at(p, g2, walk2, 0));
+                load_tile(a, p.c, tile_at<NW>(p, g2, walk2, 0));
             }
         }
         end_segment(p, lds, g, st, bad);
@@ -757,7 +782,7 @@ struct PagedSum {
 
 // EACH sums are requested at a time (behind the last one, that one again: a load that is left out would keep the others from going out together)
 template <int HD, int EACH>
-MERV_DEVICE PagedSum<HD> join_sums(const float* sums, const PagedOpen& open, int w0, int hh, int from, int step) {
+MERV_DEVICE PagedSum<HD> join_sums(const PagedAttnArgs& p, const PagedOpen& open, int w0, int hh, int from, int step) {
     constexpr int DPL = HD / 64;
     const int lane = threadIdx.x & 63;
     PagedSum<HD> s{-INFINITY, 0.f, {}};
@@ -767,7 +792,7 @@ MERV_DEVICE PagedSum<HD> join_sums(const float* sums, const PagedOpen& open, int
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
             const int v = min(w + step * e, open.last);
-            const float* x = sums + ((size_t)(v == w0 ? open.slot : 2 * v) * PAGED_HEAD_BLOCK + hh) * (HD + 4);
+            const float* x = paged_sum<HD>(p, v == w0 ? open.slot : 2 * v, hh);
             ml[e] = *(const f32x2*)(x + HD);
             if constexpr (DPL == 2) {
                 const f32x2 y = *(const f32x2*)(x + lane * 2);
@@ -814,9 +839,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs p) {
     if (hb * PAGED_HEAD_BLOCK + hh >= group || hh >= PAGED_HEAD_BLOCK) return;  // (not few: the whole workgroup)
     PagedSum<HD> s;
     if (few) {
-        s = join_sums<HD, 4>(paged_sums<HD>(p), open, w0, hh, 0, 1);
+        s = join_sums<HD, 4>(p, open, w0, hh, 0, 1);
     } else {
-        s = join_sums<HD, JOIN_MANY>(paged_sums<HD>(p), open, w0, hh, wave, 4);
+        s = join_sums<HD, JOIN_MANY>(p, open, w0, hh, wave, 4);
         if (lane == 0) {
             sm[wave] = s.m;
             sl[wave] = s.l;
@@ -879,13 +904,16 @@ hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t s) {
 }
 
 // What a call launches, from sizes alone (the rows' lengths are on the device). Where a row cannot be long, one workgroup for each pair takes it whole and
-// there is no join: up to 6 units, or 16 where there are pairs enough to fill half the card (then the longest possible row costs 22 us).
-// Measured, 16 bits, 128 dims, this and the split one: 5 units, 1 x 32 pairs 9.0 and 10.1 us, 33 x 4 9.6 and 18.1 us; 9 units, 1 x 8 13.2 and 9.7 us, 33 x 4 14.2 and
-// 17.5 us; 16 units, 33 x 4 21.9 and 23.8 us, 8 x 8 21.7 and 16.6 us.
-static bool paged_direct(long units, long pairs) { return units <= 6 || (units <= 16 && pairs >= 128); }
+// there is no join: up to 9 units, or 16 where there are pairs enough (the longest possible row then costs 18 us). Of eight waves where every pair has
+// a CU to itself and more than one round of four waves to do.
+// Measured, 16 bits, 128 dims, this and the split one: 9 units, 1 x 8 pairs 9.9 and 9.8 us, 1 x 32 10.8 and 12.2, 33 x 4 12.8 and 17.6; 16 units, 1 x 8 14.4 and 10.5 us,
+// 1 x 32 16.1 and 14.5, 8 x 8 16.1 and 16.5 (8 bits 16.0 and 13.9), 33 x 4 19.8 and 24.0. Eight and four waves: 4 units, 1 x 8 pairs 7.6 and 7.2 us; 9 units 9.9 and 11.5; 64 x 8 pairs of
+// 9 units 36.7 and 35.9.
+static bool paged_direct(long units, long pairs) { return units <= 9 || (units <= 16 && pairs >= 128); }
+static int paged_direct_waves(long units, long pairs) { return units > 4 && pairs <= 256 ? 8 : 4; }
 
 struct PagedPlan {
-    int head_blocks, workers, grid;
+    int head_blocks, workers, grid, waves;
     bool direct;
 };
 static PagedPlan paged_plan(int rows, int H, int kv_heads, long capacity) {
@@ -895,22 +923,25 @@ static PagedPlan paged_plan(int rows, int H, int kv_heads, long capacity) {
     const long pairs = (long)rows * kv_heads * pl.head_blocks, most = units * pairs;
     pl.workers = (int)(most < PAGED_MAX_WORKERS ? most : PAGED_MAX_WORKERS);
     pl.direct = paged_direct(units, pairs);
+    pl.waves = pl.direct ? paged_direct_waves(units, pairs) : 4;
     pl.grid = (int)(pl.direct || (pairs > pl.workers && pairs <= PAGED_MOST_WHOLE) ? pairs : pl.workers);
     return pl;
 }
 
 size_t paged_attention_workspace_bytes(int rows, int H, int kv_heads, int hd, long capacity) {
     const PagedPlan pl = paged_plan(rows, H, kv_heads, capacity);
-    return pl.direct ? 0 : pl.workers * (sizeof(PagedOpen) + (size_t)2 * PAGED_HEAD_BLOCK * (hd + 4) * sizeof(float));
+    const int group = H / kv_heads;
+    return pl.direct ? 0 : pl.workers * (sizeof(PagedOpen) + (size_t)2 * (group < PAGED_HEAD_BLOCK ? group : PAGED_HEAD_BLOCK) * (hd + 4) * sizeof(float));
 }
 
 template <int HD, bool E4M3>
 static hipError_t launch_paged_attention_as(const PagedAttnArgs& a, const PagedPlan& pl, hipStream_t s) {
     if (pl.direct) {
-        hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, true>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
+        if (pl.waves == 8) hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, true, 8>), dim3((unsigned)pl.grid), dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, true, 4>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, false>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attention_kernel<HD, E4M3, false, 4>), dim3((unsigned)pl.grid), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int group = a.H / a.c.kv_heads;
