@@ -618,7 +618,8 @@ MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
 //   1 row of 131072, 32 / 8 heads, 8 bits: 60 us, 4.5 TB/s, 8 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21.7 us, 2.8 TB/s
 //   1 row of 77, 16 / 2 heads: 4.5 us;  1 row of 1049, 32 / 32, 16 bits: 11.2 us
 // 512 workers: with 1024 the large call takes 363 us and 33 x 3001 takes a fifth more (twice the segments); with 256 half the loads are on their way.
-// Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit.
+// Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit (three for 8 bits: 33
+// registers spill, 33 x 3001 takes 25.9 us, 131072 75.5).
 template <int HD, bool E4M3, bool DIRECT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnArgs p) {
     static_assert(DIRECT || NW == 4, "a unit is one tile for each of four waves");

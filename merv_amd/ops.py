@@ -152,77 +152,85 @@ def gemm_mxfp8(aq, a_sc, wq, w_sc, bias=None, act="none", lscale=None, res=None,
 _PAGED_CACHE = struct.Struct("@5P7q6i")  # merv_paged_cache
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # a twentieth of torch.cuda.current_stream(dev).cuda_stream's 1.9 us
+_raw_device = torch._C._cuda_getDevice
+_E4M3, _BF16, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.int32
+
+
 def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written: bool = False):
-    """-> (the C structure, device, rows, kv_heads, head_dim, positions that a row's table can hold)."""
-    kind, shape, dev = k_pages.dtype, k_pages.shape, k_pages.device
-    if (kind is not _BF16 and kind is not _E4M3) or len(shape) != 4 or not k_pages.is_cuda:
+    """-> (the C structure, device index, rows, kv_heads, head_dim, positions that a row's table can hold)."""
+    kind, shape, st, dev = k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.get_device()
+    if (kind is not _BF16 and kind is not _E4M3) or len(st) != 4 or dev < 0:
         raise ValueError(f"{what}: expected CUDA pages [n_pages, kv_heads, page_size, head_dim] of bfloat16 or float8_e4m3fn, got "
-                         f"{kind} {tuple(shape)} on {dev}")
-    st = k_pages.stride()
-    if v_pages.dtype is not kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.device != dev:
+                         f"{kind} {tuple(shape)} on {k_pages.device}")
+    if v_pages.dtype is not kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.get_device() != dev:
         raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
     n_pages, kv_heads, page, hd = shape
-    if st[3] != 1:
+    sp, sh, ss, last = st
+    if last != 1:
         raise ValueError(f"{what}: the pages' last dimension must be contiguous")
     tst = table.stride()
-    rows, width = table.shape if len(tst) == 2 else (-1, -1)
-    if rows < 0 or table.dtype is not torch.int32 or table.device != dev or (tst[1] != 1 and width > 1):
-        raise ValueError(f"{what}: expected an int32 table [rows, width] on {dev} with contiguous rows")
-    ks = vs = 0
-    sst = (0, 0)
+    if len(tst) != 2 or table.dtype is not _I32 or table.get_device() != dev or (tst[1] != 1 and table.shape[1] > 1):
+        raise ValueError(f"{what}: expected an int32 table [rows, width] on cuda:{dev} with contiguous rows")
+    rows, width = table.shape
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    ks = vs = ssp = ssh = 0
     if kind is _E4M3:
         if k_scales is None or v_scales is None:
             raise ValueError(f"{what}: float8_e4m3fn pages need k_scales and v_scales")
         sst = k_scales.stride()
         for x in (k_scales, v_scales):
-            if x.dtype != torch.uint8 or x.shape != shape[:3] or x.device != dev or x.stride() != sst or sst[2] != 1:
-                raise ValueError(f"{what}: expected uint8 scales {tuple(shape[:3])} on {dev}, tokens contiguous, of the same strides")
-        ks, vs = k_scales.data_ptr(), v_scales.data_ptr()
-        if written and (sst[0] == 0 and n_pages > 1 or sst[1] == 0 and kv_heads > 1):
-            raise ValueError(f"{what}: scales that are written must not share memory")
+            if x.dtype is not torch.uint8 or x.shape != shape[:3] or x.get_device() != dev or x.stride() != sst or sst[2] != 1:
+                raise ValueError(f"{what}: expected uint8 scales {tuple(shape[:3])} on cuda:{dev}, tokens contiguous, of the same strides")
+        ks, vs, ssp, ssh = k_scales.data_ptr(), v_scales.data_ptr(), sst[0], sst[1]
     elif k_scales is not None or v_scales is not None:
         raise ValueError(f"{what}: bfloat16 pages take no scales")
-    if written and (st[0] == 0 and n_pages > 1 or st[1] == 0 and kv_heads > 1 or st[2] == 0):
-        raise ValueError(f"{what}: pages that are written must not share memory")
-    # the stride of a dimension of one means nothing: 0
-    c = PagedCache.from_buffer_copy(_PAGED_CACHE.pack(
-        k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), n_pages, st[0] if n_pages > 1 else 0, st[1] if kv_heads > 1 else 0, st[2],
-        sst[0] if n_pages > 1 else 0, sst[1] if kv_heads > 1 else 0, tst[0] if rows > 1 else 0, rows, width, kv_heads, hd, page,
-        KV_E4M3 if kind is _E4M3 else KV_BF16))
+    if n_pages == 1:  # the stride of a dimension of one means nothing
+        sp = ssp = 0
+    if kv_heads == 1:
+        sh = ssh = 0
+    if written and (kp == vp or ks and (ks == vs or ssp == 0 and n_pages > 1 or ssh == 0 and kv_heads > 1)
+                    or sp == 0 and n_pages > 1 or sh == 0 and kv_heads > 1 or ss == 0) and n_pages:
+        raise ValueError(f"{what}: pages and scales that are written must not share memory")
+    c = PagedCache.from_buffer_copy(_PAGED_CACHE.pack(kp, vp, ks, vs, table.data_ptr(), n_pages, sp, sh, ss, ssp, ssh, tst[0] if rows > 1 else 0, rows, width,
+                                                      kv_heads, hd, page, KV_BF16 if kind is _BF16 else KV_E4M3))
     return c, dev, rows, kv_heads, hd, width * page
 
 
-def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev, out: bool = False):
+def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev: int, out: bool = False):
     st = t.stride()
-    if t.dtype is not _BF16 or t.shape != shape or t.device != dev or st[2] != 1:
-        raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on {dev} with contiguous last dimension, got {t.dtype} "
+    if t.dtype is not _BF16 or t.shape != shape or t.get_device() != dev or st[2] != 1:
+        raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on cuda:{dev} with contiguous last dimension, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
-    s0, s1 = st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0
-    if out and (s0 == 0 and shape[0] > 1 or s1 == 0 and shape[1] > 1):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: {name} requires a gradient, and there is none: call it under torch.no_grad()")
+    s0, s1, _ = st
+    if shape[0] <= 1:
+        s0 = 0
+    elif out and s0 == 0:
+        raise ValueError(f"{what}: {name}: an output's rows must not share memory")
+    if shape[1] <= 1:
+        s1 = 0
+    elif out and s1 == 0:
         raise ValueError(f"{what}: {name}: an output's rows must not share memory")
     return t.data_ptr(), s0, s1
 
 
-def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev) -> int:
+def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev: int) -> int:
     if t is None:
         return 0
-    if t.dtype is not torch.int32 or t.shape != (n,) or t.device != dev or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not _I32 or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # a hundredth of torch.cuda.current_stream(dev).cuda_stream's 1.9 us
-_E4M3, _BF16 = torch.float8_e4m3fn, torch.bfloat16
-
-
-def _launch_on(dev, call, what: str, *args) -> None:
+def _launch_on(dev: int, call, what: str, *args) -> None:
     """call(*args, stream) on the device's current stream; the device is made current where it is not (its null stream has no device of its own)."""
-    i = dev.index
-    if torch._C._cuda_getDevice() == i:
-        rc = call(*args, _raw_stream(i))
+    if _raw_device() == dev:
+        rc = call(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = call(*args, _raw_stream(i))
+            rc = call(*args, _raw_stream(dev))
     if rc:
         check(rc, what)
 
@@ -250,8 +258,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     if cos is not None and sin is not None:
         cst, cshape = cos.stride(), cos.shape
         for t in (cos, sin):
-            if t.dtype != torch.bfloat16 or t.shape != cshape or len(cshape) != 2 or cshape[1] != hd or t.device != dev or t.stride() != cst or cst[1] != 1:
-                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {hd}] on {dev} with contiguous rows, of the same strides")
+            if t.dtype is not _BF16 or t.shape != cshape or len(cst) != 2 or cshape[1] != hd or t.get_device() != dev or t.stride() != cst or cst[1] != 1:
+                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {hd}] on cuda:{dev} with contiguous rows, of the same strides")
         rope = (cos.data_ptr(), sin.data_ptr(), cshape[0], cst[0] if cshape[0] > 1 else hd)
     elif cos is not None or sin is not None or q is not None:
         raise ValueError(f"{what}: cos and sin come together, and q needs them")
@@ -286,9 +294,9 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.
     shape = (total, kv_heads, hd)
     off_p, start_p = _paged_ints(what, "offsets", offsets, rows + 1, dev), _paged_ints(what, "start", start, rows, dev)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        k_out = torch.empty(shape, dtype=_BF16, device=k_pages.device)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        v_out = torch.empty(shape, dtype=_BF16, device=k_pages.device)
     ko, vo = _paged_rows(what, "k_out", k_out, shape, dev, True), _paged_rows(what, "v_out", v_out, shape, dev, True)
     _launch_on(dev, _lib.load().merv_paged_cache_read, what, cache, *ko, *vo, off_p, start_p, total)
     return k_out, v_out
@@ -313,11 +321,11 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if out is None:
         out = torch.empty_like(q)
     orow = _paged_rows(what, "out", out, qshape, dev, True)
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if return_lse else None
     lib = _lib.load()
     # a workspace of its own for each call (and each captured graph): nothing is shared by calls that run at the same time
     nbytes = lib.merv_paged_decode_attention_workspace_bytes(rows, heads, kv_heads, hd, capacity)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _launch_on(dev, lib.merv_paged_decode_attention, what, cache, *qr, *orow, 0 if lse is None else lse.data_ptr(), lens_p, heads, int(window),
                hd**-0.5 if scale is None else float(scale), 0 if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out

@@ -490,3 +490,51 @@ def test_nothing_to_do(dev):
     q = torch.ones(2, 2, 64, dtype=torch.bfloat16, device=dev)
     out = ops.paged_decode_attention(q, pool.k, pool.v, torch.empty(2, 0, dtype=torch.int32, device=dev), i32([0, 0], dev))
     assert (out == 0).all()
+
+
+def test_the_wrappers_refuse(dev):
+    """What the tensors alone show, before any launch; nothing is written."""
+    from merv_amd import ops
+    pool = P.Pool([20, 9], 2, 64, 16, "bf16", dev)
+    table, n = pool.table.to(dev), i32([20, 9], dev)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=dev)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=dev)
+    cos = torch.zeros(30, 64, dtype=torch.bfloat16, device=dev)
+    e4 = pool.k.to(torch.float8_e4m3fn)
+    sc = torch.zeros(pool.k.shape[:3], dtype=torch.uint8, device=dev)
+
+    def write(k=k, v=k, kp=pool.k, vp=pool.v, table=table, start=n, off=None, **kw):
+        ops.paged_cache_write(k, v, kp, vp, table, start, off, **kw)
+
+    def read(start=None, off=i32([0, 1, 2], dev), total=2, **kw):
+        ops.paged_cache_read(pool.k, pool.v, table, start, off, total, **kw)
+
+    def att(q=q, kp=pool.k, vp=pool.v, table=table, lens=n, **kw):
+        ops.paged_decode_attention(q, kp, vp, table, lens, **kw)
+
+    grad = k.clone().requires_grad_()
+    shared = pool.k[:1].expand(4, -1, -1, -1)
+    cases = [
+        (write, dict(kp=pool.k.float(), vp=pool.v.float()), "float8_e4m3fn"), (write, dict(kp=pool.k[0], vp=pool.v[0]), "CUDA pages"),
+        (write, dict(vp=pool.v.transpose(1, 2)), "v_pages"), (write, dict(kp=e4, vp=e4.clone()), "need k_scales"), (write, dict(k_scales=sc, v_scales=sc), "no scales"),
+        (write, dict(kp=e4, vp=e4.clone(), k_scales=sc[:1], v_scales=sc[:1]), "uint8 scales"), (write, dict(vp=pool.k), "share memory"),
+        (write, dict(kp=e4, vp=e4.clone(), k_scales=sc, v_scales=sc), "share memory"), (write, dict(kp=shared, vp=pool.v[:1].expand(4, -1, -1, -1)), "share memory"),
+        (write, dict(table=table.long()), "int32 table"), (write, dict(table=table.cpu()), "int32 table"), (write, dict(k=k[:1], v=k[:1]), "one token for each row"),
+        (write, dict(k=k.float()), "k: expected"), (write, dict(v=k[:, :1]), "v: expected"), (write, dict(start=n.long()), "start: expected"),
+        (write, dict(start=n[:1]), "start: expected"), (write, dict(off=n), "offsets: expected"), (write, dict(q=q), "q needs them"), (write, dict(cos=cos), "come together"),
+        (write, dict(q=q, cos=cos, sin=cos[:5]), "rotary tables"), (write, dict(q=q, cos=cos.float(), sin=cos.float()), "rotary tables"),
+        (write, dict(q=q[:1], cos=cos, sin=cos), "q: expected"), (write, dict(q_out=q), "q_out needs q"), (write, dict(k=grad), "requires a gradient"),
+        (write, dict(q=q, cos=cos, sin=cos, q_out=q[:, :1].expand(-1, 4, -1)), "share memory"), (write, dict(k_out=k.cpu()), "k_out: expected"),
+        (write, dict(k=torch.zeros(2, 2, 68, dtype=torch.bfloat16, device=dev)[..., 4:]), "16-byte"),
+        (read, dict(total=-1), "negative"), (read, dict(off=None), "offsets"), (read, dict(off=n), "offsets: expected"), (read, dict(k_out=k.float()), "k_out: expected"),
+        (att, dict(q=q[:1]), "q: expected"), (att, dict(q=q[:, :3]), "multiple of 2"), (att, dict(q=q[:, :, :32]), "q: expected"), (att, dict(q=q.half()), "q: expected"),
+        (att, dict(window=-1), "window"), (att, dict(lens=n.long()), "lens: expected"), (att, dict(out=q[:, :1].expand(-1, 4, -1)), "share memory"),
+        (att, dict(lens=n.cpu()), "lens: expected"), (att, dict(kp=pool.k[:, :, :12], vp=pool.v[:, :, :12]), "page_size"),
+    ]
+    before = [pool.k.clone(), pool.v.clone()]
+    for call, kw, msg in cases:
+        with pytest.raises(ValueError, match=msg):
+            call(**kw)
+    assert same(pool.k, before[0]) and same(pool.v, before[1])
+    with torch.no_grad():
+        write(k=grad, v=k, start=i32([0, 0], dev))
