@@ -623,7 +623,7 @@ MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
 template <int HD, bool E4M3, bool DIRECT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnArgs p) {
     static_assert(DIRECT || NW == 4, "a unit is one tile for each of four waves");
-    __shared__ PagedLds<HD, NW> lds;
+    __shared__ __attribute__((aligned(16))) PagedLds<HD, NW> lds;
     const int pairs = p.c.kv_heads * p.head_blocks;
     PagedSegment g;
     int x = 0, end = 0, w = 0;  // units of the line: behind this segment, behind this worker; the worker

@@ -90,6 +90,7 @@ class PagedDecoder(StaticDecoder):
         self.pos = torch.full((batch,), -1, dtype=torch.int32, device=self.dev)  # the position that a row's next token takes
         self.held: List[int] = [0] * batch  # the same on the host
         self.room: List[int] = [0] * batch  # positions that a row has pages for
+        self.captured_weights = ()
         cfg = self.cfg
         win, kinds = getattr(cfg, "sliding_window", None), getattr(cfg, "layer_types", None)
         if not getattr(cfg, "use_sliding_window", True):
@@ -197,11 +198,15 @@ class PagedDecoder(StaticDecoder):
         news = self._rows(inputs_embeds, "prefill")
         if max(news) >= self.max_len:
             raise ValueError(f"prefill: prompts of {news} tokens, the cache holds {self.max_len} positions a row")
-        self.room = [self.max_len if room is None else min(self.max_len, n + room) for n in news]
-        self.cache.assign(self.room)
-        self.held = [0] * self.B
+        room = [self.max_len if room is None else min(self.max_len, n + room) for n in news]
+        self.cache.assign(room)
+        self.room, self.held = room, [0] * self.B
         with torch.cuda.device(self.dev):
-            return self._known_tokens(inputs_embeds, news)
+            logits = self._known_tokens(inputs_embeds, news)
+        where = tuple(p.data_ptr() for p in self.m.parameters())
+        if where != self.captured_weights:  # a step captured before a parameter's storage was replaced reads the old one
+            self.graph, self.captured_weights = None, where
+        return logits
 
     @torch.inference_mode()
     def extend(self, inputs_embeds) -> torch.Tensor:

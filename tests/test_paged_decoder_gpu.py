@@ -173,6 +173,28 @@ def test_generation_of_a_ragged_batch(dev, kv):
     assert got.shape == (3, 6)
 
 
+def test_replaced_weights_are_seen_by_the_next_prompt(dev):
+    """A captured step holds addresses: after a parameter's storage is replaced, by one decoder's leave or another's, the next prompt captures anew."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb, t = prompts([9, 4], 256, dev), torch.tensor([5, 9], device=dev)
+    decs = [PagedDecoder(bb.llm, 64, 2) for _ in range(2)]
+    for d in decs:
+        d.prefill(emb)
+        d.decode(t)
+    with torch.no_grad():
+        for lyr in bb.llm.model.layers:
+            for lin in (lyr.self_attn.q_proj, lyr.self_attn.o_proj, lyr.mlp.up_proj):
+                lin.weight.data = (lin.weight * 1.5).clone()
+    for d in decs:
+        d.prefill(emb)
+        got = d.decode(t)
+        for b in range(2):
+            row = Formula(bb, d.cos, d.sin, "bf16")
+            row.run(emb[b])
+            assert rel_l2(got[b], row.run(bb.embed_input_ids(t)[b:b + 1])) < TOL["bf16"]
+
+
 def test_static_generation_is_untouched_by_the_paged_one(dev):
     bb = backbone(dev)
     emb = prompts([30], 256, dev)[0][None]

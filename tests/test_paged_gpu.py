@@ -297,6 +297,35 @@ def test_attention_joins_of_many_parts(dev):
     check_attention(dev, [4000 + 100 * i for i in range(14)], 5, 5, 64, 256, "bf16")
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_attention_split_over_blocks_of_heads(dev, fmt):
+    """20 query heads a key head (two blocks of 16 columns) and 128 dims, a row over many workers beside short ones."""
+    check_attention(dev, [5000, 3, 0, 130], 40, 2, 128, 32, fmt)
+
+
+def test_attention_thousands_of_rows(dev):
+    """More rows than a lane of the prefix sum has one of, short in a large table: left whole (2000 pairs), and shared out (4500, over the limit for that)."""
+    check_attention(dev, [(i * 7) % 30 for i in range(2000)], 1, 1, 64, 16, "bf16", width=100)
+    check_attention(dev, [(i * 11) % 20 for i in range(4500)], 1, 1, 64, 16, "bf16", width=100)
+
+
+def test_attention_strided_operands(dev):
+    """Queries that are columns of a projection, an output that is columns of something wider, a table that is part of a larger one, every other row."""
+    from merv_amd import ops
+    lens, H, Hkv, hd = [300, 17, 1400], 8, 2, 128
+    pool = P.Pool(lens, Hkv, hd, 32, "e4m3", dev)
+    kk, vv = pool.fill(*P.rows_like(lens, Hkv, hd, 1))
+    wide = torch.randn(6, 3 * H * hd, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(dev)
+    q = wide[::2, H * hd:2 * H * hd].view(3, H, hd)
+    out = torch.full((3, 2, H, hd), 7.0, dtype=torch.bfloat16, device=dev)
+    big = torch.full((6, pool.width + 5), -9, dtype=torch.int32, device=dev)
+    big[::2, 2:2 + pool.width] = pool.table.to(dev)
+    got, lse = ops.paged_decode_attention(q, pool.k, pool.v, big[::2, 2:2 + pool.width], i32(lens, dev), out=out[:, 1], return_lse=True, **pool.scales())
+    assert got.data_ptr() == out[:, 1].data_ptr() and (out[:, 0] == 7).all()
+    want, want_l, tol, tol_l = P.attention(q.cpu(), kk, vv, hd**-0.5)
+    assert ((got.cpu().to(P.F64) - want).abs() <= tol).all() and ((lse.cpu().to(P.F64) - want_l).abs() <= tol_l).all()
+
+
 def test_attention_peaked_and_flat(dev):
     """Scores of some hundreds, where all weight is on one position, and a scale of zero, where all weigh the same."""
     check_attention(dev, [700, 40], 4, 2, 128, 32, "bf16", q_gain=30.0)
