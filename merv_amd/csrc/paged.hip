@@ -831,8 +831,9 @@ template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs p) {
     constexpr int DPL = HD / 64;
     __shared__ float sm[4], sl[4], so[4][HD];
-    const PagedOpen open = ((const PagedOpen*)p.ws)[blockIdx.x];
-    const int w0 = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // (one long row's pairs begin in every 64th worker or so: in a row of workgroups that is one XCD)
+    const int w0 = xcd_remap(blockIdx.x, p.workers), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedOpen open = ((const PagedOpen*)p.ws)[w0];
     const bool few = open.last - w0 < JOIN_MANY;
     if (open.last < 0 || (few && (blockIdx.y & 3))) return;
     const int group = p.H / p.c.kv_heads, hkv = open.pair / p.head_blocks, hb = open.pair - hkv * p.head_blocks;
