@@ -599,7 +599,8 @@ MERV_DEVICE void write_unseen(const PagedAttnArgs& p, int row, int h, int d) {  
 
 // what a worker leaves beside its sums: word of the pair that goes on behind it, and the results of every p.workers-th row that has no units
 template <int HD>
-MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
+MERV_DEVICE void end_worker(const PagedAttnArgs& p, PagedOpen open, const PagedShare& share) {
+    if (open.last >= 0) open.last = paged_owner(share, open.last);  // (until here: the pair's last unit)
     if (threadIdx.x == 0) ((PagedOpen*)p.ws)[blockIdx.x] = open;
     for (int r = blockIdx.x; r < p.c.rows; r += p.workers)
         if (span_of(p, r).units == 0)
@@ -615,7 +616,7 @@ MERV_DEVICE void end_worker(const PagedAttnArgs& p, const PagedOpen& open) {
 //
 // Bound by HBM where the call is large, by its chain of round trips (length, pages, keys and values, sums) where it is small. Measured, 128 dims:
 //   96 rows of 2458 .. 8192 positions, 32 / 8 heads, 16 bits: 352 us, 5.87 TB/s of keys and values (a copy of 1 GiB on this card: 5.05)
-//   1 row of 131072, 32 / 8 heads, 8 bits: 60 us, 4.5 TB/s, 8 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21.7 us, 2.8 TB/s
+//   1 row of 131072, 32 / 8 heads, 8 bits: 58 us, 4.7 TB/s, 6 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21.7 us, 2.8 TB/s
 //   1 row of 77, 16 / 2 heads: 4.5 us;  1 row of 1049, 32 / 32, 16 bits: 11.2 us
 // 512 workers: with 1024 the large call takes 363 us and 33 x 3001 takes a fifth more (twice the segments); with 256 half the loads are on their way.
 // Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit (three for 8 bits: 33
@@ -633,9 +634,10 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
     bool whole = DIRECT;  // one pair of one row
     if constexpr (!DIRECT) {
         const int rows = p.c.rows, per = (rows + 63) / 64, lane = threadIdx.x & 63, r0 = min(rows, lane * per), r1 = min(rows, r0 + per);
-        int mine = 0, most = 0;
+        int mine = 0, most = 0, len = 0;
         for (int r = r0; r < r1; ++r) {
-            const int n = span_of_len(p, p.lens[r]).units;
+            len = p.lens[r];
+            const int n = span_of_len(p, len).units;
             mine += n;
             most = max(most, n);
         }
@@ -648,7 +650,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
             if (threadIdx.x == 0 && w < p.workers) ((PagedOpen*)p.ws)[w] = open;
             if (w >= rows * pairs) return;
         } else if (w >= share.workers) {
-            if (w < p.workers) end_worker<HD>(p, open);
+            if (w < p.workers) end_worker<HD>(p, open, share);
             return;
         } else {
             x = paged_start(share, w);
@@ -657,8 +659,8 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
             const int at = __ffsll(__ballot(x >= (sum - mine) * pairs && x < sum * pairs)) - 1;
             int before = __builtin_amdgcn_readlane(sum - mine, at);
             g.row = at * per;
-            PagedSpan sp = span_of(p, g.row);
-            while (x >= (before + sp.units) * pairs) {
+            PagedSpan sp = per == 1 ? span_of_len(p, __builtin_amdgcn_readlane(len, at)) : span_of(p, g.row);
+            while (x >= (before + sp.units) * pairs) {  // (per > 1)
                 before += sp.units;
                 sp = span_of(p, ++g.row);
             }
@@ -668,7 +670,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
             g.u = in_row - g.pair * sp.units;
             g.n = min(g.units - g.u, end - x);
             g.slot = g.n == g.units ? -1 : paged_slot(w, true);
-            if (g.u == 0 && g.n < g.units) open = PagedOpen{g.row, g.pair, g.slot, paged_owner(share, x + g.units - 1)};
+            if (g.u == 0 && g.n < g.units) open = PagedOpen{g.row, g.pair, g.slot, x + g.units - 1};
             x += g.n;
         }
     }
@@ -716,7 +718,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
                 }
                 g2.n = min(g2.units, end - x);
                 g2.slot = g2.n == g2.units ? -1 : paged_slot(w, false);
-                if (g2.n < g2.units) open = PagedOpen{g2.row, g2.pair, g2.slot, paged_owner(share, x + g2.units - 1)};
+                if (g2.n < g2.units) open = PagedOpen{g2.row, g2.pair, g2.slot, x + g2.units - 1};
                 x += g2.n;
                 walk2 = begin_walk<NW, false>(p, g2, 0);
             }
@@ -768,7 +770,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
         bad = bad2;
     }
     if constexpr (!DIRECT)
-        if (!whole) end_worker<HD>(p, open);
+        if (!whole) end_worker<HD>(p, open, share);
 }
 
 // Joins the partial sums of the pair that begins in a worker and ends in a later one, if there is one; the worker left word of it (PagedOpen), so nothing
