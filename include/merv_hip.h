@@ -462,7 +462,8 @@ int merv_map_pool_attention(const void *kv, const float *q, void *out, int32_t n
  *  stands for code * 2^(byte - 127). table[row * table_stride + i] is the page that holds positions i * page_size .. of a row; entries no call reaches
  *  may hold anything. Device-side integers are never trusted with an address: see each call for what a bad one does.
  *  Limits: head_dim 64 or 128; page_size a power of two from 16 to 1024; page and row pointers 16-byte aligned with strides that are multiples of 8 (bf16) or 16
- *  (e4m3) elements, scale pointers 4-byte aligned with strides that are multiples of 4.
+ *  (e4m3) elements, scale pointers 4-byte aligned with strides that are multiples of 4. A write takes up to 2^28 vectors (keys, values and queries), a
+ *  read 2^27 keys, an attention under 2^22 rows x heads, 2^30 positions a row and under 2^31 units of 128 positions over all rows and heads.
  */
 enum { MERV_KV_BF16 = 0, MERV_KV_E4M3 = 1 };
 typedef struct merv_paged_cache {

@@ -1180,8 +1180,8 @@ extern "C" int merv_paged_cache_write(const merv_paged_cache* cache, const void*
                                       const int32_t* offsets, const int32_t* start, int32_t T, int32_t heads, void* stream_) {
     PagedWriteArgs a{};
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
-    MERV_CHECK(T >= 0 && heads >= 0 && heads <= 65536 && cache->kv_heads <= 65536 && (int64_t)T * (2 * (int64_t)cache->kv_heads + heads) < (1LL << 36),
-               "merv_paged_cache_write: bad geometry");
+    MERV_CHECK(T >= 0 && heads >= 0, "merv_paged_cache_write: bad geometry");
+    MERV_CHECK((int64_t)T * (2 * (int64_t)cache->kv_heads + heads) <= (1LL << 28), "merv_paged_cache_write: at most 2^28 keys, values and queries a call");
     MERV_CHECK(offsets || T == cache->rows, "merv_paged_cache_write: without offsets there is one token for each row");
     if (T == 0) return 0;
     MERV_CHECK(k && v && start, "merv_paged_cache_write: null argument");
@@ -1210,7 +1210,8 @@ extern "C" int merv_paged_cache_read(const merv_paged_cache* cache, void* k_out,
                                      void* stream_) {
     PagedReadArgs a{};
     if (int rc = paged_cache_args(cache, &a.c)) return rc;
-    MERV_CHECK(T >= 0 && cache->kv_heads <= 65536 && (int64_t)T * cache->kv_heads < (1LL << 35), "merv_paged_cache_read: bad geometry");
+    MERV_CHECK(T >= 0, "merv_paged_cache_read: bad geometry");
+    MERV_CHECK((int64_t)T * cache->kv_heads <= (1LL << 27), "merv_paged_cache_read: at most 2^27 keys a call");
     if (T == 0) return 0;
     MERV_CHECK(k_out && v_out && offsets, "merv_paged_cache_read: null argument");
     MERV_CHECK(paged_rows_ok(k_out, k_out_stride, k_out_head_stride) && paged_rows_ok(v_out, v_out_stride, v_out_head_stride),
@@ -1237,9 +1238,10 @@ extern "C" int merv_paged_decode_attention(const merv_paged_cache* cache, const 
     MERV_CHECK(heads > 0 && heads % cache->kv_heads == 0, "merv_paged_decode_attention: heads must be a multiple of kv_heads");
     if (cache->rows == 0) return 0;
     const int64_t capacity = (int64_t)cache->table_width * cache->page_size;
-    MERV_CHECK(capacity <= (1LL << 30) && cache->stride_token >= 0 && cache->stride_token < (1LL << 26) &&
+    MERV_CHECK(capacity <= (1LL << 30) && cache->stride_token >= 0 && cache->stride_token < (1LL << 26) && (int64_t)cache->rows * heads < (1LL << 22) &&
                    (capacity / PAGED_UNIT + 1) * cache->rows * heads < (1LL << 31),
-               "merv_paged_decode_attention: at most 2^30 positions a row, 2^31 units of 128 positions over all rows and heads, a token stride under 2^26");
+               "merv_paged_decode_attention: at most 2^22 rows times heads, 2^30 positions a row, 2^31 units of 128 positions over all rows and heads, a token "
+               "stride under 2^26");
     MERV_CHECK(q && out && lens, "merv_paged_decode_attention: null argument");
     MERV_CHECK(paged_rows_ok(q, q_stride, q_head_stride) && paged_rows_ok(out, out_stride, out_head_stride),
                "merv_paged_decode_attention: rows must be 16-byte aligned with strides that are multiples of 8");

@@ -165,6 +165,8 @@ def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written
                          f"{kind} {tuple(shape)} on {k_pages.device}")
     if v_pages.dtype is not kind or v_pages.shape != shape or v_pages.stride() != st or v_pages.get_device() != dev:
         raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
+    if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
+        raise ValueError(f"{what}: the pages require a gradient, and there is none: call it under torch.no_grad()")
     n_pages, kv_heads, page, hd = shape
     sp, sh, ss, last = st
     if last != 1:
@@ -243,13 +245,16 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     cos, sin [positions, head_dim] bf16 are given. Token t is row b's where offsets[b] <= t < offsets[b + 1] (int32 [rows + 1]; None: one token a
     row, t = b), at position start[b] + t - offsets[b]; rows with start[b] < 0 and tokens behind offsets[rows] are left alone, in every output. Returns
     the rotated queries (q_out, or a new tensor; q_out=q rotates in place), None without q; k_out takes the rotated keys as well. float8_e4m3fn pages:
-    quantised with one power-of-two scale for each token and head (k_scales, v_scales); what is not finite becomes NaN."""
+    quantised with one power-of-two scale for each token and head (k_scales, v_scales); what is not finite becomes NaN. Two tokens of a call must not lie in
+    the same place of a page (rows may share pages that are only read)."""
     what = "paged_cache_write"
     cache, dev, rows, kv_heads, hd, _ = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales, True)
     if k.dim() != 3:
         raise ValueError(f"{what}: k: expected [tokens, kv_heads, head_dim], got {tuple(k.shape)}")
     T = k.shape[0]
     shape = (T, kv_heads, hd)
+    if T > 1 << 28:
+        raise ValueError(f"{what}: at most 2^28 tokens a call")
     if offsets is None and T != rows:
         raise ValueError(f"{what}: without offsets there is one token for each row: {T} tokens, {rows} rows")
     kr, vr = _paged_rows(what, "k", k, shape, dev), _paged_rows(what, "v", v, shape, dev)
@@ -289,8 +294,8 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.
     what = "paged_cache_read"
     cache, dev, rows, kv_heads, hd, _ = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
     total = int(total)
-    if total < 0 or offsets is None:
-        raise ValueError(f"{what}: total must not be negative, and offsets are needed")
+    if not 0 <= total <= 1 << 27 or offsets is None:
+        raise ValueError(f"{what}: total must not be negative or over 2^27, and offsets are needed")
     shape = (total, kv_heads, hd)
     off_p, start_p = _paged_ints(what, "offsets", offsets, rows + 1, dev), _paged_ints(what, "start", start, rows, dev)
     if k_out is None:

@@ -235,6 +235,7 @@ class PagedDecoder(StaticDecoder):
         """token [batch]: each row's token at its position -> logits behind it [batch, vocab] (fp32)."""
         if not all(self.held) or any(s >= r for s, r in zip(self.held, self.room)):
             raise ValueError(f"decode: rows hold {self.held} positions, with room for {self.room}")
-        out = super().decode(token, use_graph)
+        with torch.cuda.device(self.dev):  # a capture is of the current device's stream
+            out = super().decode(token, use_graph)
         self.held = [n + 1 for n in self.held]
         return out

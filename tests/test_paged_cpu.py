@@ -59,6 +59,24 @@ def test_bad_calls_are_refused():
                       ((64, 250, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0), "16-byte"), ((72, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0), "16-byte")]:
         with pytest.raises(ValueError, match=msg):
             _lib.check(lib.merv_paged_decode_attention(c, *args), "attention")
+    # calls that a launch could not cover
+    big = _cache(rows=1 << 20, kv_heads=1 << 11, n_pages=0, k_pages=0, v_pages=0)
+    edge = _cache(rows=1, kv_heads=1, n_pages=0, k_pages=0, v_pages=0)  # 2^32 threads, one more than a launch has
+    for rc in (lambda: lib.merv_paged_cache_write(edge, 64, 128, 64, 64, 128, 64, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 64, 64, (1 << 28) - 1, 0, 0),
+               lambda: lib.merv_paged_cache_read(edge, 64, 128, 64, 64, 128, 64, 64, 0, (1 << 28) - 1, 0),
+               lambda: lib.merv_paged_cache_write(big, 64, 128, 64, 64, 128, 64, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 64, 64, 1 << 18, 0, 0),
+               lambda: lib.merv_paged_cache_read(big, 64, 128, 64, 64, 128, 64, 64, 0, 1 << 18, 0),
+               lambda: lib.merv_paged_decode_attention(big, 64, 256, 64, 64, 256, 64, 0, 64, 1 << 11, 0, 1.0, 4096, 1 << 30, 0),
+               lambda: lib.merv_paged_decode_attention(_cache(table_width=1 << 27), 64, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0),
+               lambda: lib.merv_paged_decode_attention(_cache(table_width=1 << 24, rows=1 << 10), 64, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0),
+               lambda: lib.merv_paged_decode_attention(_cache(stride_token=1 << 26), 64, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0)):
+        with pytest.raises(ValueError, match="at most"):
+            _lib.check(rc(), "paged")
+    with pytest.raises(ValueError, match="workspace too small"):  # 2048 positions a row, few pairs: shared out, which takes a workspace
+        _lib.check(lib.merv_paged_decode_attention(_cache(table_width=128), 64, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 4096, 100, 0), "attention")
+    need = lib.merv_paged_decode_attention_workspace_bytes(3, 4, 2, 64, 2048)
+    assert need == 3 * 2 * 16 * (16 + 2 * 2 * 68 * 4) and lib.merv_paged_decode_attention_workspace_bytes(3, 4, 2, 64, 512) == 0
+    assert lib.merv_paged_decode_attention_workspace_bytes(3, 5, 2, 64, 2048) == 0
     with pytest.raises(ValueError, match="null"):
         _lib.check(lib.merv_paged_decode_attention(C.POINTER(_lib.PagedCache)(), 64, 256, 64, 64, 256, 64, 0, 64, 4, 0, 1.0, 0, 0, 0), "attention")
 

@@ -303,10 +303,12 @@ def test_attention_split_over_blocks_of_heads(dev, fmt):
     check_attention(dev, [5000, 3, 0, 130], 40, 2, 128, 32, fmt)
 
 
-def test_attention_thousands_of_rows(dev):
-    """More rows than a lane of the prefix sum has one of, short in a large table: left whole (2000 pairs), and shared out (4500, over the limit for that)."""
-    check_attention(dev, [(i * 7) % 30 for i in range(2000)], 1, 1, 64, 16, "bf16", width=100)
-    check_attention(dev, [(i * 11) % 20 for i in range(4500)], 1, 1, 64, 16, "bf16", width=100)
+@pytest.mark.parametrize("width", [100, 200])
+def test_attention_thousands_of_rows(dev, width):
+    """More rows than a lane of the prefix sum has one of, short in a large table. At 100 pages a row one workgroup a row without a plan; at 200 the plan
+    leaves 2000 rows whole and shares 4500 out."""
+    check_attention(dev, [(i * 7) % 30 for i in range(2000)], 1, 1, 64, 16, "bf16", width=width)
+    check_attention(dev, [(i * 11) % 20 for i in range(4500)], 1, 1, 64, 16, "bf16", width=width)
 
 
 def test_attention_strided_operands(dev):
@@ -332,10 +334,11 @@ def test_attention_peaked_and_flat(dev):
     check_attention(dev, [700, 40], 4, 2, 128, 32, "bf16", scale=0.0)
 
 
-def test_attention_bad_rows_are_nan_alone(dev):
+@pytest.mark.parametrize("width", [None, 200])  # left whole, and shared out
+def test_attention_bad_rows_are_nan_alone(dev, width):
     from merv_amd import ops
     lens = [300, 300, 300, 300, 0]
-    pool = P.Pool(lens, 2, 64, 16, "bf16", dev)
+    pool = P.Pool(lens, 2, 64, 16, "bf16", dev, width=width)
     pool.fill(*P.rows_like(lens, 2, 64, 1))
     table = pool.table.clone()
     table[1, 9], table[2, 0] = pool.k.shape[0], -1
@@ -521,6 +524,26 @@ def test_nothing_to_do(dev):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("width", [4, 200])
+def test_a_pool_without_pages(dev, fmt, width):
+    """Every position is one without a page: nothing is stored, queries and keys come out as NaN, what is read is NaN; a row of length 0 is as ever."""
+    from merv_amd import ops
+    kind = torch.bfloat16 if fmt == "bf16" else torch.float8_e4m3fn
+    pages = [torch.empty(0, 2, 16, 64, dtype=kind, device=dev) for _ in range(2)]
+    sc = {} if fmt == "bf16" else {n: torch.empty(0, 2, 16, dtype=torch.uint8, device=dev) for n in ("k_scales", "v_scales")}
+    table = torch.zeros(3, width, dtype=torch.int32, device=dev)
+    k, q = torch.ones(3, 2, 64, dtype=torch.bfloat16, device=dev), torch.ones(3, 4, 64, dtype=torch.bfloat16, device=dev)
+    cos, sin = (t.to(dev) for t in tables(64, 64))
+    k_out = torch.zeros_like(k)
+    q_out = ops.paged_cache_write(k, k, *pages, table, i32([0, 20, 3], dev), q=q, cos=cos, sin=sin, k_out=k_out, **sc)
+    assert torch.isnan(q_out).all() and torch.isnan(k_out).all()
+    kk, vv = ops.paged_cache_read(*pages, table, None, i32([0, 2, 2, 5], dev), 5, **sc)
+    assert torch.isnan(kk).all() and torch.isnan(vv).all()
+    out, lse = ops.paged_decode_attention(q, *pages, table, i32([40, 0, 64], dev), return_lse=True, **sc)
+    assert torch.isnan(out[[0, 2]]).all() and torch.isnan(lse[[0, 2]]).all() and (out[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
 def test_the_wrappers_refuse(dev):
     """What the tensors alone show, before any launch; nothing is written."""
     from merv_amd import ops
@@ -554,6 +577,8 @@ def test_the_wrappers_refuse(dev):
         (write, dict(q=q, cos=cos, sin=cos[:5]), "rotary tables"), (write, dict(q=q, cos=cos.float(), sin=cos.float()), "rotary tables"),
         (write, dict(q=q[:1], cos=cos, sin=cos), "q: expected"), (write, dict(q_out=q), "q_out needs q"), (write, dict(k=grad), "requires a gradient"),
         (write, dict(q=q, cos=cos, sin=cos, q_out=q[:, :1].expand(-1, 4, -1)), "share memory"), (write, dict(k_out=k.cpu()), "k_out: expected"),
+        (write, dict(kp=pool.k.clone().requires_grad_()), "require a gradient"), (att, dict(vp=pool.v.clone().requires_grad_()), "require a gradient"),
+        (write, dict(k=k[:1].expand((1 << 28) + 1, 2, 64), v=k[:1].expand((1 << 28) + 1, 2, 64), off=i32([0, 1, 2], dev)), "at most"), (read, dict(total=1 << 32), "over"),
         (write, dict(k=torch.zeros(2, 2, 68, dtype=torch.bfloat16, device=dev)[..., 4:]), "16-byte"),
         (read, dict(total=-1), "negative"), (read, dict(off=None), "offsets"), (read, dict(off=n), "offsets: expected"), (read, dict(k_out=k.float()), "k_out: expected"),
         (att, dict(q=q[:1]), "q: expected"), (att, dict(q=q[:, :3]), "multiple of 2"), (att, dict(q=q[:, :, :32]), "q: expected"), (att, dict(q=q.half()), "q: expected"),
