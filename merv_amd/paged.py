@@ -181,9 +181,12 @@ class PagedDecoder(StaticDecoder):
                     kb, vb = k[lo:hi], v[lo:hi]
                 j, i = torch.arange(ends[b], device=self.dev)[None], torch.arange(self.held[b], ends[b], device=self.dev)[:, None]
                 mask = (j <= i) & (j > i - win) if win else j <= i
-                o = F.scaled_dot_product_attention(q[lo:hi].transpose(0, 1)[None], kb.transpose(0, 1)[None], vb.transpose(0, 1)[None], attn_mask=mask[None, None],
+                qb = q[lo:hi]
+                if H != Hkv:  # a mask and shared heads: batched products, in 32 bits by name (16-bit ones with a transposed operand are not to be relied on)
+                    qb, kb, vb = qb.float(), kb.float(), vb.float()
+                o = F.scaled_dot_product_attention(qb.transpose(0, 1)[None], kb.transpose(0, 1)[None], vb.transpose(0, 1)[None], attn_mask=mask[None, None],
                                                    enable_gqa=H != Hkv)
-                out[lo:hi] = o[0].transpose(0, 1).reshape(n, H * hd)
+                out[lo:hi] = o[0].transpose(0, 1).reshape(n, H * hd)  # (rounds to bf16)
             return out
 
         x = self._layers(x, attend)
