@@ -247,9 +247,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
 // V's operand wants 8 positions of one dim in a lane; a lane loads 8 positions x HD/16 neighbouring dims in whole lines and transposes them in registers
 // (v_perm_b32), row r of product dt being dim r * HD/16 + dt. K's operand wants a key in a lane: loaded so, a wave's 64 16-byte pieces lie in 16 lines of memory
 // (62 GB/s a CU); loaded in whole lines and turned in the wave's own corner of LDS, 80 (16 bits; one row of 4096 positions, unsplit, 38.6 and 30.2 us).
-// Scores, maximum, sum and output are fp32. A weight p is used as the sum of two bf16 numbers, p cut off and the rest rounded (2^-15 relative: one bf16
-// alone would add as much error as the output's own rounding); where values may be infinite the rest is kept above zero (by 2^-20 p), so that it
-// neither turns an infinity round nor makes it NaN. The running maximum moves only when a score exceeds it by 2^6: the rescaling of the 32 output
+// Scores, maximum, sum and output are fp32, and so are the weights: the 24 bits of a p are three bf16 numbers of 8 each (split_weight), whose products with
+// bf16 values are exact in fp32. Two of them (2^-17 off) turned 0.3 - 0.6 % of the outputs to the other side of their rounding. The running maximum moves only when a score exceeds it by 2^6: the rescaling of the 32 output
 // registers is then rare, and nothing overflows that would not without it.
 // e4m3 codes become bf16 exactly; a key's power of two multiplies its score, a value's its weight.
 constexpr float RAISE = 6.f;
@@ -332,6 +331,20 @@ struct PagedState {  // of a wave: lane l has head l % 16
     f32x4 o[HD / 16];
 };
 
+// p >= 0 as the sum of three bf16 numbers (the upper halves of x), exactly: p cut off behind 8 bits, the rest cut off, the rest of that, which has 8 bits left.
+// POSITIVE, where values may be infinite: all three parts of a p > 0 are over zero, so that none turns an infinity round or makes it NaN. For that the number
+// before p is cut off instead of p: what is left is over zero and, where p itself had 8 bits only, a power of two.
+template <bool POSITIVE>
+MERV_DEVICE void split_weight(float p, uint32_t (&x)[3]) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const uint32_t bits = __float_as_uint(p);
+        x[n] = (POSITIVE ? __builtin_elementwise_sub_sat(bits, 1u) : bits) & 0xffff0000u;
+        p -= __uint_as_float(x[n]);
+    }
+    x[2] = __float_as_uint(p);
+}
+
 template <int HD, bool E4M3>
 MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int tok, int lo, int len, char* room) {
     typedef PagedTile<HD, E4M3> Tile;
@@ -395,7 +408,7 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
         for (int d = 0; d < HD / 16; ++d) st.o[d] *= a;
     }
     const float base = st.m == -INFINITY ? 0.f : st.m;
-    uint32_t hi[4], lo_[4];
+    u32x4 part[3];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
         float p[4];
@@ -407,16 +420,13 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            const float p0 = p[2 * w], p1 = p[2 * w + 1];
-            const uint32_t h0 = __float_as_uint(p0) & 0xffff0000u, h1 = __float_as_uint(p1) & 0xffff0000u;
-            float l0 = p0 - __uint_as_float(h0), l1 = p1 - __uint_as_float(h1);
-            if constexpr (!E4M3) l0 = fmaxf(l0, p0 * 0x1p-20f), l1 = fmaxf(l1, p1 * 0x1p-20f);
-            hi[tt * 2 + w] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
-            lo_[tt * 2 + w] = pack2bf(l0, l1);
+            uint32_t x[3], y[3];
+            split_weight<!E4M3>(p[2 * w], x);
+            split_weight<!E4M3>(p[2 * w + 1], y);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) part[n][tt * 2 + w] = __builtin_amdgcn_perm(y[n], x[n], 0x07060302u);
         }
     }
-    const bf16x8 ph = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
-    const bf16x8 pl = __builtin_bit_cast(bf16x8, u32x4{lo_[0], lo_[1], lo_[2], lo_[3]});
 #pragma unroll
     for (int w = 0; w < Tile::DV / 2; ++w) {  // dims 2w and 2w + 1 of the lane's
         uint32_t x[8];
@@ -431,10 +441,12 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
             even[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
             odd[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
         }
-        st.o[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), ph, st.o[2 * w], 0, 0, 0);
-        st.o[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), ph, st.o[2 * w + 1], 0, 0, 0);
-        st.o[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pl, st.o[2 * w], 0, 0, 0);
-        st.o[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pl, st.o[2 * w + 1], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            const bf16x8 pn = __builtin_bit_cast(bf16x8, part[n]);
+            st.o[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pn, st.o[2 * w], 0, 0, 0);
+            st.o[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pn, st.o[2 * w + 1], 0, 0, 0);
+        }
     }
 }
 

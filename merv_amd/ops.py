@@ -313,7 +313,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """Attention of one token for each row, q [rows, heads, head_dim] bf16, over positions max(0, lens[b] - window) .. lens[b] - 1 of the row's pages
     (window 0: all of them; kv head = head // (heads // kv_heads); scale None: head_dim^-0.5). Returns out, or (out, lse [rows, heads] fp32, the
     natural logarithm of the softmax's sum). A row of length 0 gives zeros and -inf; a length over the table's capacity or a bad page gives
-    that row NaN. Sums, softmax and the weights of the values are held in fp32 (the weights as two bf16 numbers); rounded to bf16 once, at the end."""
+    that row NaN. Sums, softmax and the weights of the values are held in fp32; rounded to bf16 once, at the end."""
     what = "paged_decode_attention"
     cache, dev, rows, kv_heads, hd, capacity = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
     qshape = q.shape
