@@ -473,7 +473,7 @@ struct PagedAttnArgs {
     long q_st, q_sh, o_st, o_sh;
     int H, window;     // window 0: all positions
     float scale;
-    int head_blocks, workers;  // set by the launch
+    int head_blocks, workers, shift;  // set by the launch
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
 size_t paged_attention_workspace_bytes(int rows, int H, int kv_heads, int hd, long capacity);

@@ -248,10 +248,13 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
 // (v_perm_b32), row r of product dt being dim r * HD/16 + dt. K's operand wants a key in a lane: loaded so, a wave's 64 16-byte pieces lie in 16 lines of memory
 // (62 GB/s a CU); loaded in whole lines and turned in the wave's own corner of LDS, 80 (16 bits; one row of 4096 positions, unsplit, 38.6 and 30.2 us).
 // Scores, maximum, sum and output are fp32, and so are the weights: the 24 bits of a p are three bf16 numbers of 8 each (split_weight), whose products with
-// bf16 values are exact in fp32. Two of them (2^-17 off) turned 0.3 - 0.6 % of the outputs to the other side of their rounding. The running maximum moves only when a score exceeds it by 2^6: the rescaling of the 32 output
-// registers is then rare, and nothing overflows that would not without it.
+// bf16 values are exact in fp32. Two of them (2^-17 off) turned 0.3 - 0.6 % of the outputs to the other side of their rounding.
+// The running maximum moves only when a weight would exceed 2^RAISE: the rescaling of the 32 output registers is then rare. A row's weights may so add up to
+// 2^RAISE times its positions; they and their sum are used 2^-shift times that, `shift` chosen from the longest possible row, so that a sum
+// of weighted values never exceeds the largest value: the result is finite where the formula's is. (Weights and values whose product is under
+// 2^(shift - 126), with a shift of 20 for 16384 positions, lose bits to fp32's smallest numbers.)
 // e4m3 codes become bf16 exactly; a key's power of two multiplies its score, a value's its weight.
-constexpr float RAISE = 6.f;
+constexpr int RAISE = 6;
 
 template <int HD, bool E4M3>
 struct PagedTile {  // 32 positions of one head in a wave's registers
@@ -346,7 +349,8 @@ MERV_DEVICE void split_weight(float p, uint32_t (&x)[3]) {
 }
 
 template <int HD, bool E4M3>
-MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int tok, int lo, int len, char* room) {
+MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16x8 (&q)[HD / 32], float scale2, int shift, int tok, int lo, int len,
+                          char* room) {
     typedef PagedTile<HD, E4M3> Tile;
     constexpr int CPR = Tile::CPR, RPL = 16 / CPR;  // keys in 256 bytes of LDS
     const int lane = threadIdx.x & 63, tg = lane >> 4;
@@ -399,7 +403,7 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = max_over_rows(top);
-    if (__any(top > st.m + RAISE)) {
+    if (__any(top > st.m + (float)RAISE)) {
         const float m = fmaxf(st.m, top);
         const float a = __builtin_amdgcn_exp2f(st.m - (m == -INFINITY ? 0.f : m));
         st.m = m;
@@ -408,6 +412,7 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
         for (int d = 0; d < HD / 16; ++d) st.o[d] *= a;
     }
     const float base = st.m == -INFINITY ? 0.f : st.m;
+    const float down = __uint_as_float((uint32_t)(127 - shift) << 23);
     u32x4 part[3];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt) {
@@ -416,7 +421,8 @@ MERV_DEVICE void use_tile(PagedState<HD>& st, PagedTile<HD, E4M3>& t, const bf16
         for (int i = 0; i < 4; ++i) {
             p[i] = __builtin_amdgcn_exp2f(s[tt][i] - base);
             st.l += p[i];
-            if constexpr (E4M3) p[i] = ldexpf(p[i], (int)((t.vs[tt] >> (8 * i)) & 0xff) - 127);
+            if constexpr (E4M3) p[i] = ldexpf(p[i], (int)((t.vs[tt] >> (8 * i)) & 0xff) - 127 - shift);
+            else p[i] *= down;
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -559,7 +565,7 @@ MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD, NW>& lds, cons
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int group = p.H / p.c.kv_heads, hkv = g.pair / p.head_blocks, hb = g.pair - hkv * p.head_blocks;
     const int h0 = hkv * group + hb * PAGED_HEAD_BLOCK, heads = min(PAGED_HEAD_BLOCK, group - hb * PAGED_HEAD_BLOCK);
-    st.l = sum_over_rows(st.l);
+    st.l = ldexpf(sum_over_rows(st.l), -p.shift);  // as the weights
     if (__any(bad)) st.l = __builtin_nanf("");
     const int h = lane & 15;
     if (h < heads) {
@@ -592,7 +598,7 @@ MERV_DEVICE void end_segment(const PagedAttnArgs& p, PagedLds<HD, NW>& lds, cons
         if (g.slot < 0) {
             const u32x2 o = {pack2bf(O[0] / L, O[1] / L), pack2bf(O[2] / L, O[3] / L)};
             *(u32x2*)(p.out + (long)g.row * p.o_st + (long)(h0 + hh) * p.o_sh + d) = o;
-            if (p.lse && d == 0) p.lse[(long)g.row * p.H + h0 + hh] = (M + __builtin_amdgcn_logf(L)) * LN2;
+            if (p.lse && d == 0) p.lse[(long)g.row * p.H + h0 + hh] = (M + __builtin_amdgcn_logf(ldexpf(L, p.shift))) * LN2;
         } else {
             float* ws = paged_sum<HD>(p, g.slot, hh);
             *(f32x4*)(ws + d) = O;
@@ -756,14 +762,14 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_attention_kernel(PagedAttnAr
         for (int i = 0; i < walk.tiles;) {
             load_tile(b, p.c, behind(i));
             __builtin_amdgcn_sched_barrier(0);  // all of the next tile is requested before the first wait for this one
-            use_tile(st, a, q, scale2, walk.first + i * (32 * NW), g.lo, g.len, room);
+            use_tile(st, a, q, scale2, p.shift, walk.first + i * (32 * NW), g.lo, g.len, room);
             if (++i == walk.tiles) {
                 in_b = true;
                 break;
             }
             load_tile(a, p.c, behind(i));
             __builtin_amdgcn_sched_barrier(0);
-            use_tile(st, b, q, scale2, walk.first + i * (32 * NW), g.lo, g.len, room);
+            use_tile(st, b, q, scale2, p.shift, walk.first + i * (32 * NW), g.lo, g.len, room);
             ++i;
         }
         if (more) {
@@ -879,7 +885,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs p) {
     bf16_t* out = p.out + (long)open.row * p.o_st + (long)h * p.o_sh + lane * DPL;
     if constexpr (DPL == 2) *(uint32_t*)out = pack2bf(s.o[0] / s.l, s.o[1] / s.l);
     else *out = f2bf(s.o[0] / s.l);
-    if (p.lse && lane == 0) p.lse[(long)open.row * p.H + h] = (s.m + __builtin_amdgcn_logf(s.l)) * LN2;
+    if (p.lse && lane == 0) p.lse[(long)open.row * p.H + h] = (s.m + __builtin_amdgcn_logf(ldexpf(s.l, p.shift))) * LN2;
 }
 
 }  // namespace
@@ -971,6 +977,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs& args, hipStream_t s) {
     const PagedPlan pl = paged_plan(a.c.rows, a.H, a.c.kv_heads, (long)a.c.table_width << a.c.page_log2);
     a.head_blocks = pl.head_blocks;
     a.workers = pl.workers;
+    const long capacity = (long)a.c.table_width << a.c.page_log2, most = a.window > 0 && a.window < capacity ? a.window : capacity;
+    for (a.shift = RAISE; (1L << (a.shift - RAISE)) < most;) ++a.shift;  // (most <= 2^30)
     if (a.c.hd == 128) return a.c.e4m3 ? launch_paged_attention_as<128, true>(a, pl, s) : launch_paged_attention_as<128, false>(a, pl, s);
     if (a.c.hd == 64) return a.c.e4m3 ? launch_paged_attention_as<64, true>(a, pl, s) : launch_paged_attention_as<64, false>(a, pl, s);
     return hipErrorInvalidValue;

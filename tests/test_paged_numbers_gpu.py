@@ -51,3 +51,29 @@ def test_weights_are_held_in_32_bits(dev, fmt, n, width):
     tol = (5 * p[:, None] * v[at[0]].abs() + 14 * terms) * 2.0**-24 / total + 2.0**-8 * want.abs()
     over = (out - want).abs() / tol
     assert bool((over <= 1).all()), (float(over.max()), float((over > 1).double().mean()))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("width", [None, 300])  # a workgroup for each pair (None: or for the longest rows shared out, too), and shared out
+def test_large_values_stay_finite(dev, fmt, width):
+    """Values near the largest number, in every position: the result is a mean of them. Scores grow along the row by a little (under what moves the running
+    maximum), in one head, and are alike in the other."""
+    from merv_amd import ops
+    hd, lens = 64, [1, 33, 200, 1100, 2300]
+    k, v = P.rows_like(lens, 1, hd, 3)
+    for x in k:
+        x.zero_()
+        x[:, 0, 0] = torch.linspace(0, 4, x.shape[0]).to(torch.bfloat16)  # score 4 = 5.8 in base 2
+    for i, x in enumerate(v):
+        x[:] = (3.0e38 * torch.where(torch.arange(hd) % 2 == 0, 1.0, -1.0)).to(torch.bfloat16)
+        x[:, 0, 10:20] = torch.randn(x.shape[0], 10, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16)
+        x[:, 0, 20:30] *= 2.0**-120
+    q = torch.zeros(len(lens), 2, hd, dtype=torch.bfloat16)
+    q[:, 0, 0] = 1.0
+    pool = P.Pool(lens, 1, hd, 16, fmt, dev, width=width)
+    kk, vv = pool.fill(k, v)
+    want, want_l, tol, tol_l = P.attention(q, kk, vv, 1.0)
+    out, lse = ops.paged_decode_attention(q.to(dev), pool.k, pool.v, pool.table.to(dev), i32(lens, dev), scale=1.0, return_lse=True, **pool.scales())
+    out = out.cpu().to(P.F64)
+    assert torch.isfinite(out).all()
+    assert ((out - want).abs() <= tol).all() and ((lse.cpu().to(P.F64) - want_l).abs() <= tol_l).all()
