@@ -77,3 +77,35 @@ def test_large_values_stay_finite(dev, fmt, width):
     out = out.cpu().to(P.F64)
     assert torch.isfinite(out).all()
     assert ((out - want).abs() <= tol).all() and ((lse.cpu().to(P.F64) - want_l).abs() <= tol_l).all()
+
+
+@pytest.mark.parametrize("fmt,hd", [("bf16", 128), ("bf16", 64), ("e4m3", 128), ("e4m3", 64)])
+@pytest.mark.parametrize("window", [0, 5000])
+def test_long_stretches_of_one_row(dev, fmt, hd, window):
+    """A worker that takes more than 32 units of one pair looks up page numbers anew every 32 tiles. 600 rows of 4096 .. 8200 positions (32, 33, 64 and 65
+    units) on the same pages, two pairs each: over 100 units a worker, so that whole rows lie in it. A row whose table has one bad page, before, at
+    or behind such a border, is NaN, and no other is."""
+    from merv_amd import ops
+    H, Hkv, page, B = 4, 2, 16, 600
+    kinds = [8200, 4096, 4097, 8192, 4224, 4225, 8191, 5000]
+    pool = P.Pool([max(kinds)], Hkv, hd, page, fmt, dev, seed=2)
+    kk, vv = pool.fill(*P.rows_like([max(kinds)], Hkv, hd, 1))
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(len(kinds), H, hd, generator=g).to(torch.bfloat16)
+    want, want_l, tol, tol_l = P.attention(q, [kk[0][:n] for n in kinds], [vv[0][:n] for n in kinds], hd**-0.5, window)
+    which = torch.arange(B) % len(kinds)
+    lens = torch.tensor(kinds)[which]
+    table = pool.table.expand(B, -1).clone()
+    bad = {40: 4095, 41: 4095, 80: 4096, 81: 4095, 160: 8191, 163: 8191, 240: 8199, 299: 4999, 300: 4223}  # row: position (all seen)
+    for n, (b, pos) in enumerate(bad.items()):
+        assert int(lens[b]) - (window or 10**6) <= pos < int(lens[b])
+        table[b, pos // page] = [-1, pool.k.shape[0], 2**31 - 1][n % 3]
+    out, lse = ops.paged_decode_attention(q[which].to(dev), pool.k, pool.v, table.to(dev), i32(lens.tolist(), dev), window=window, return_lse=True,
+                                          **pool.scales())
+    out, lse = out.cpu().to(P.F64), lse.cpu().to(P.F64)
+    rows = torch.tensor(sorted(bad))
+    assert torch.isnan(out[rows]).all() and torch.isnan(lse[rows]).all()
+    good = torch.ones(B, dtype=torch.bool)
+    good[rows] = False
+    w = which[good]
+    assert ((out[good] - want[w]).abs() <= tol[w]).all() and ((lse[good] - want_l[w]).abs() <= tol_l[w]).all()
