@@ -90,7 +90,8 @@ class PagedDecoder(StaticDecoder):
         self.pos = torch.full((batch,), -1, dtype=torch.int32, device=self.dev)  # the position that a row's next token takes
         self.held: List[int] = [0] * batch  # the same on the host
         self.room: List[int] = [0] * batch  # positions that a row has pages for
-        self.captured_weights = ()
+        self.holders = self._holders()
+        self.captured_weights: List[int] = []  # where the captured step's parameters lie
         cfg = self.cfg
         win, kinds = getattr(cfg, "sliding_window", None), getattr(cfg, "layer_types", None)
         if not getattr(cfg, "use_sliding_window", True):
@@ -99,6 +100,19 @@ class PagedDecoder(StaticDecoder):
 
     def _allocate(self) -> None:
         self.cache = PagedKVCache(self.cfg.num_hidden_layers, self.B, self.max_len, self.Hkv, self.hd, self.dev, **self.cache_args)
+
+    def _holders(self) -> List[torch.nn.Module]:
+        return [mod for mod in self.m.modules() if mod._parameters]
+
+    def _drop_stale_step(self) -> None:
+        """A captured step holds its parameters' addresses: one captured before a parameter or its storage was replaced is not replayed. Looked at before each
+        step (120 us of the host's time for 32 layers, behind a step of milliseconds); modules that were replaced themselves are seen at the next prompt."""
+        if self.graph is not None and self._addresses() != self.captured_weights:
+            torch.cuda.synchronize(self.dev)  # a replay may be under way
+            self.graph = None
+
+    def _addresses(self) -> List[int]:
+        return [p.data_ptr() for mod in self.holders for p in mod._parameters.values() if p is not None]
 
     def _layers(self, x: torch.Tensor, attend) -> torch.Tensor:
         """The decoder stack on x [T, D] (updated in place): attend(li, q, k, v) -> [T, H * hd] with q / k / v column ranges of one projection. Returns x."""
@@ -145,6 +159,7 @@ class PagedDecoder(StaticDecoder):
     def _known_tokens(self, embeds: Sequence[torch.Tensor], news: List[int]) -> torch.Tensor:
         """Runs known tokens, packed row behind row, behind the self.held positions of each; returns the logits behind each row's last one."""
         H, Hkv, hd, cache = self.H, self.Hkv, self.hd, self.cache
+        self.holders = self._holders()
         offsets, ends = [0], []
         for n in news:
             offsets.append(offsets[-1] + n)
@@ -206,9 +221,6 @@ class PagedDecoder(StaticDecoder):
         self.room, self.held = room, [0] * self.B
         with torch.cuda.device(self.dev):
             logits = self._known_tokens(inputs_embeds, news)
-        where = tuple(p.data_ptr() for p in self.m.parameters())
-        if where != self.captured_weights:  # a step captured before a parameter's storage was replaced reads the old one
-            self.graph, self.captured_weights = None, where
         return logits
 
     @torch.inference_mode()
@@ -239,6 +251,11 @@ class PagedDecoder(StaticDecoder):
         if not all(self.held) or any(s >= r for s, r in zip(self.held, self.room)):
             raise ValueError(f"decode: rows hold {self.held} positions, with room for {self.room}")
         with torch.cuda.device(self.dev):  # a capture is of the current device's stream
+            if use_graph:
+                self._drop_stale_step()
+            captured = self.graph
             out = super().decode(token, use_graph)
+            if self.graph is not captured:
+                self.captured_weights = self._addresses()
         self.held = [n + 1 for n in self.held]
         return out

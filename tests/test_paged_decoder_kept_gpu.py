@@ -1,0 +1,87 @@
+"""GPU: what a PagedDecoder keeps from call to call: its captured step, its pool of pages."""
+import pytest
+import torch
+
+from conftest import rel_l2
+from test_paged_decoder_gpu import TOL, Formula, backbone, prompts
+
+pytestmark = pytest.mark.gpu
+
+
+def replaced(bb, factor):
+    """Other storages for all but q / k / v (whose replacement is seen by their own check); -> the old ones, to put back and to keep alive."""
+    old = []
+    with torch.no_grad():
+        for p in [bb.llm.model.norm.weight] + [lin.weight for lyr in bb.llm.model.layers for lin in (lyr.self_attn.o_proj, lyr.mlp.up_proj, lyr.post_attention_layernorm)]:
+            old.append((p, p.data))
+            p.data = (p * factor).clone()
+    return old
+
+
+def put_back(old):
+    for p, data in old:
+        p.data = data
+
+
+def test_replaced_weights_are_seen_behind_a_held_prompt(dev):
+    """prefill, decode (captures), other weights, extend, decode: the step behind extend() uses what extend() used."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb, more, t = prompts([9, 4], 256, dev), prompts([3, 6], 256, dev, 5), torch.tensor([5, 9], device=dev)
+    dec = PagedDecoder(bb.llm, 64, 2)
+    dec.prefill(emb)
+    dec.decode(t)
+    rows = [Formula(bb, dec.cos, dec.sin, "bf16") for _ in range(2)]
+    for b, row in enumerate(rows):
+        row.run(emb[b])
+        row.run(bb.embed_input_ids(t)[b:b + 1])
+    old = replaced(bb, 1.5)
+    got = dec.extend(more)
+    last = dec.decode(t).clone()
+    for b, row in enumerate(rows):
+        assert rel_l2(got[b], row.run(more[b])) < TOL["bf16"]
+        assert rel_l2(last[b], row.run(bb.embed_input_ids(t)[b:b + 1])) < TOL["bf16"]
+    put_back(old)
+
+
+@pytest.mark.parametrize("between", ["prefill", "nothing"])
+def test_a_step_captured_with_other_weights_is_not_replayed(dev, between):
+    """Weights A at the prompt, B at the first step (captured), A again: the next step, behind a new prompt or not, uses A."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb, t = prompts([9, 4], 256, dev), torch.tensor([5, 9], device=dev)
+    dec = PagedDecoder(bb.llm, 64, 2)
+    dec.prefill(emb)
+    old = replaced(bb, 1.5)
+    kept = [(p, p.data) for p, _ in old]  # B's storages stay alive
+    dec.decode(t)
+    put_back(old)
+    if between == "prefill":
+        dec.prefill(emb)
+        got = dec.decode(t)
+        want = PagedDecoder(bb.llm, 64, 2)
+        want.prefill(emb)
+        assert torch.equal(got, want.decode(t, use_graph=False))
+    else:
+        got = dec.decode(t).clone()
+        dec.held = [n - 1 for n in dec.held]
+        dec.pos -= 1  # the same step again, not captured
+        assert torch.equal(got, dec.decode(t, use_graph=False))
+    assert len(kept) == len(old)
+
+
+def test_a_replaced_parameter_is_seen(dev):
+    """Another Parameter object in a module's place, with a captured step alive."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb, t = prompts([9, 4], 256, dev), torch.tensor([5, 9], device=dev)
+    dec = PagedDecoder(bb.llm, 64, 2)
+    dec.prefill(emb)
+    dec.decode(t)
+    kept = bb.llm.lm_head.weight
+    bb.llm.lm_head.weight = torch.nn.Parameter((kept * -1.0).detach(), requires_grad=False)
+    dec.prefill(emb)
+    got = dec.decode(t).clone()
+    want = PagedDecoder(bb.llm, 64, 2)
+    want.prefill(emb)
+    assert torch.equal(got, want.decode(t, use_graph=False))
