@@ -58,6 +58,26 @@ class PagedKVCache:
         return d if self.k_scales is None else dict(d, k_scales=self.k_scales[i], v_scales=self.v_scales[i])
 
 
+SCORES = 1 << 28  # of one product in known_attention: 1 GiB
+
+
+def known_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int) -> torch.Tensor:
+    """q [n, H, hd] at the last n of the positions of k, v [positions, Hkv, hd], each over what is at or before it (the newest `window` of that, 0: all) -> [n, H, hd].
+    In 32 bits, rounded to q's type at the end: under a mask SDPA may take its batched products, whose 16-bit form with a transposed right operand has faulted the
+    GPU with this torch build. Queries in blocks, so that no product has more than SCORES scores."""
+    n, H, hd = q.shape
+    past, out = k.shape[0] - n, torch.empty_like(q, memory_format=torch.contiguous_format)
+    each = max(1, SCORES // (H * k.shape[0]))
+    for a in range(0, n, each):
+        b = min(n, a + each)
+        lo = max(0, past + a - window + 1) if window else 0
+        i, j = torch.arange(past + a, past + b, device=q.device)[:, None], torch.arange(lo, past + b, device=q.device)[None]
+        mask = (j <= i) & (j > i - window) if window else j <= i
+        qb, kb, vb = (x.float().transpose(0, 1)[None] for x in (q[a:b], k[lo:past + b], v[lo:past + b]))
+        out[a:b] = F.scaled_dot_product_attention(qb, kb, vb, attn_mask=mask[None, None], enable_gqa=H != k.shape[1])[0].transpose(0, 1)
+    return out
+
+
 class PagedDecoder(StaticDecoder):
     """Prefill and token-by-token decoding of `batch` rows of any prompt lengths. prefill(prompts), then decode(tokens) once a token, as the other decoders;
     extend(more) puts further known tokens behind what the rows hold (a second question on the same clip) without running the first ones again.
@@ -194,14 +214,7 @@ class PagedDecoder(StaticDecoder):
                     kb[self.held[b]:], vb[self.held[b]:] = k[lo:hi], v[lo:hi]  # its own keys as they are
                 else:
                     kb, vb = k[lo:hi], v[lo:hi]
-                j, i = torch.arange(ends[b], device=self.dev)[None], torch.arange(self.held[b], ends[b], device=self.dev)[:, None]
-                mask = (j <= i) & (j > i - win) if win else j <= i
-                qb = q[lo:hi]
-                if H != Hkv:  # a mask and shared heads: batched products, in 32 bits by name (16-bit ones with a transposed operand are not to be relied on)
-                    qb, kb, vb = qb.float(), kb.float(), vb.float()
-                o = F.scaled_dot_product_attention(qb.transpose(0, 1)[None], kb.transpose(0, 1)[None], vb.transpose(0, 1)[None], attn_mask=mask[None, None],
-                                                   enable_gqa=H != Hkv)
-                out[lo:hi] = o[0].transpose(0, 1).reshape(n, H * hd)  # (rounds to bf16)
+                out[lo:hi] = known_attention(q[lo:hi], kb, vb, win).view(n, H * hd)
             return out
 
         x = self._layers(x, attend)

@@ -85,3 +85,19 @@ def test_a_replaced_parameter_is_seen(dev):
     want = PagedDecoder(bb.llm, 64, 2)
     want.prefill(emb)
     assert torch.equal(got, want.decode(t, use_graph=False))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hidden,window", [(2, 2, 256, None), (4, 4, 256, None), (2, 2, 256, 24), (4, 2, 256, 24), (4, 4, 256, 24)])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_known_tokens_of_heads_of_their_own(dev, fmt, heads, kv_heads, hidden, window):
+    """Prompts, steps and further tokens where each query head has its key head (and where two share one), 64 and 128 dims, with and without a window."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev, "mistral" if window else "llama", heads, kv_heads, hidden, **(dict(sliding_window=window) if window else {}))
+    dec = PagedDecoder(bb.llm, 128, 2, fmt=fmt, page_size=32)
+    first, second, t = prompts([40, 3], hidden, dev, 1), prompts([5, 41], hidden, dev, 2), torch.tensor([5, 9], device=dev)
+    rows = [Formula(bb, dec.cos, dec.sin, fmt, window or 0) for _ in range(2)]
+    got = [dec.prefill(first), dec.decode(t).clone(), dec.extend(second), dec.decode(t).clone()]
+    for b, row in enumerate(rows):
+        e = bb.embed_input_ids(t)[b:b + 1]
+        for x, known in zip(got, (first[b], e, second[b], e)):
+            assert rel_l2(x[b], row.run(known)) < TOL[fmt]
