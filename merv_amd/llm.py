@@ -172,7 +172,7 @@ class LlamaBackbone:
         top_k = int(top_k or 0)
         dec = None
         if kv_cache != "static":
-            from .paged import PagedDecoder
+            from .paged import PagedDecoder, pool_pages
             need = max(e.shape[0] for e in inputs_embeds) + max_new_tokens + 1
             if need > self.config.max_position_embeddings:
                 raise ValueError(f"{need} positions are needed, the model has {self.config.max_position_embeddings}")
@@ -180,9 +180,10 @@ class LlamaBackbone:
             key = (bucket, rows, kv_cache)
             if not hasattr(self, "_decoders"):
                 self._decoders = {}
-            if key not in self._decoders:
+            pages = pool_pages([e.shape[0] + max_new_tokens + 1 for e in inputs_embeds], bucket)
+            if key not in self._decoders or self._decoders[key].cache.n_pages < pages:
                 self._decoders.clear()
-                self._decoders[key] = PagedDecoder(self.llm, bucket, rows, fmt="e4m3" if kv_cache == "paged-e4m3" else "bf16")
+                self._decoders[key] = PagedDecoder(self.llm, bucket, rows, fmt="e4m3" if kv_cache == "paged-e4m3" else "bf16", n_pages=pages)
             dec = self._decoders[key]
             logits = dec.prefill(inputs_embeds, room=max_new_tokens + 1)
             step = lambda tok: dec.decode(tok, use_graph=use_graph)

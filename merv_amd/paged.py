@@ -17,6 +17,14 @@ from ._lib import check, ptr
 from .llm import HipDecoder, StaticDecoder
 
 
+def pool_pages(lengths: Sequence[int], max_len: int, page_size: int = 64) -> int:
+    """Pages of a pool for rows of `lengths` positions (at most max_len each), rounded up to whole 256 positions a row, so that a pool also serves batches a little longer."""
+    width = -(-max_len // page_size)
+    each = len(lengths) * max(1, 256 // page_size)
+    need = sum(min(width, -(-int(n) // page_size)) for n in lengths)
+    return min(len(lengths) * width, -(-need // each) * each) if need else 0
+
+
 class PagedKVCache:
     """Pages of all layers and the table that says which of them a row's positions lie in (one table for all layers). fmt "bf16", or "e4m3": 8-bit
     numbers with a power-of-two scale for each token and head. `n_pages` None: enough for every row at `max_len` positions."""
@@ -84,7 +92,9 @@ class PagedDecoder(StaticDecoder):
 
     Projections and the MLP's products are library GEMMs over all rows' tokens, everything between them library calls of libmerv_hip.so: norms,
     rotary embedding + cache write (+ quantisation), attention, silu * up. A prompt attends to its own unquantised keys; what is read back
-    from the cache, by decode() and extend(), is what the cache holds. A step is captured once in a hipGraph and replayed."""
+    from the cache, by decode() and extend(), is what the cache holds. A step is captured once in a hipGraph and replayed.
+
+    `n_pages`: the pool that all rows share (None: enough for every row at max_len). A batch that needs more is refused by prefill()."""
 
     # q / k / v as one product, the module's parameters re-homed once as HipDecoder does it
     fuse_qkv, _qkv_fused = HipDecoder.fuse_qkv, HipDecoder._qkv_fused
@@ -99,10 +109,10 @@ class PagedDecoder(StaticDecoder):
         return (hd in (64, 128) and p.is_cuda and p.dtype == torch.bfloat16 and not mlp_bias and cfg.hidden_size % 8 == 0 and cfg.hidden_size <= 8192
                 and cfg.intermediate_size % 8 == 0)
 
-    def __init__(self, hf_model, max_len: int, batch: int = 1, fmt: str = "bf16", page_size: int = 64) -> None:
+    def __init__(self, hf_model, max_len: int, batch: int = 1, fmt: str = "bf16", page_size: int = 64, n_pages: Optional[int] = None) -> None:
         if not self.supports(hf_model):
             raise ValueError("PagedDecoder: a bfloat16 CUDA module with head_dim 64 or 128, at most 8192 hidden units and no MLP biases is needed")
-        self.cache_args = dict(fmt=fmt, page_size=page_size)
+        self.cache_args = dict(fmt=fmt, page_size=page_size, n_pages=n_pages)
         super().__init__(hf_model, max_len, batch)
         self.lib = _lib.load()
         for lyr in hf_model.model.layers:

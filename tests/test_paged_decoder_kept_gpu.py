@@ -101,3 +101,28 @@ def test_known_tokens_of_heads_of_their_own(dev, fmt, heads, kv_heads, hidden, w
         e = bb.embed_input_ids(t)[b:b + 1]
         for x, known in zip(got, (first[b], e, second[b], e)):
             assert rel_l2(x[b], row.run(known)) < TOL[fmt]
+
+
+@pytest.mark.parametrize("kv", ["paged", "paged-e4m3"])
+def test_a_ragged_batch_takes_the_pages_it_needs(dev, kv):
+    """One long prompt beside short ones: a pool for their sum, not for the longest in every row; a batch that needs more gets a larger one, a smaller one the same."""
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb = prompts([700] + [9] * 7, 256, dev)
+    ids = bb.generate_from_embeds(emb, max_new_tokens=6, kv_cache=kv)
+    dec, = bb._decoders.values()
+    assert dec.cache.n_pages == 32 and dec.cache.k.shape[1] == 32  # 12 + 7 pages of 64, rounded up; 8 x 12 for eight rows of 768
+    full = PagedDecoder(bb.llm, 768, 8, fmt="e4m3" if kv.endswith("e4m3") else "bf16")
+    assert full.cache.n_pages == 96
+    tok = full.prefill(emb).argmax(-1)
+    for i in range(6):
+        assert torch.equal(ids[:, i], tok)
+        tok = full.decode(tok).argmax(-1)
+    bb.generate_from_embeds(prompts([600] * 4 + [9] * 4, 256, dev), max_new_tokens=100, kv_cache=kv)
+    larger, = bb._decoders.values()
+    assert larger is not dec and larger.cache.n_pages == 64
+    assert torch.equal(ids, bb.generate_from_embeds(emb, max_new_tokens=6, kv_cache=kv))
+    assert bb._decoders[next(iter(bb._decoders))] is larger
+    small = PagedDecoder(bb.llm, 768, 8, n_pages=18)
+    with pytest.raises(ValueError, match="pages needed"):
+        small.prefill(emb, room=7)

@@ -39,3 +39,21 @@ def test_known_attention(monkeypatch, H, Hkv, n, past, window, scores):
             x = vd[lo:hi, h // (H // Hkv)]
             want = p @ x
             assert ((out[i, h].double() - want).abs() <= 2.0**-16 * (p @ x.abs()) + 2.0**-8 * want.abs()).all()
+
+
+def test_a_pool_is_as_large_as_its_rows_need():
+    from merv_amd.paged import PagedKVCache, pool_pages
+    assert pool_pages([8000] + [50] * 31, 8192) == 256  # 125 + 31 pages, rounded up to 4 a row on the average; 4096 for 32 rows of 8192
+    assert pool_pages([1082] * 8, 1280) == 8 * 20  # rows of one length: all of the table
+    assert pool_pages([1000, 1000], 1000) == 2 * 16  # never more than the rows' tables name
+    assert pool_pages([10**6, 1], 256) == 8 and pool_pages([0, 0], 256) == 0 and pool_pages([], 256) == 0
+    assert pool_pages([100], 4096, 1024) == 1 and pool_pages([1, 1, 1], 4096, 16) == 48
+    import random
+    rng = random.Random(1)
+    for _ in range(200):
+        page, rows, most = rng.choice([16, 64, 1024]), rng.randint(1, 20), rng.randint(1, 5000)
+        lengths = [rng.randint(0, most) for _ in range(rows)]
+        c = PagedKVCache(1, rows, most, 1, 64, "cpu", page_size=page, n_pages=0)
+        need = sum(-(-n // page) for n in lengths)
+        got = pool_pages(lengths, most, page)
+        assert need <= got <= rows * c.width and got < need + rows * max(1, 256 // page)
