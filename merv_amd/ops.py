@@ -152,8 +152,8 @@ def gemm_mxfp8(aq, a_sc, wq, w_sc, bias=None, act="none", lscale=None, res=None,
 _PAGED_CACHE = struct.Struct("@5P7q6i")  # merv_paged_cache
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # a twentieth of torch.cuda.current_stream(dev).cuda_stream's 1.9 us
-_raw_device = torch._C._cuda_getDevice
+# a twentieth of torch.cuda.current_stream(dev).cuda_stream's 1.9 us; a torch without a GPU has neither (there the calls refuse their tensors before they need them)
+_raw_stream, _raw_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
 _E4M3, _BF16, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.int32
 
 
