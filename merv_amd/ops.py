@@ -9,6 +9,7 @@ import struct
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import ACT, DT_BF16, DT_F32, KV_BF16, KV_E4M3, PagedCache, check, current_stream_ptr, ptr
@@ -157,6 +158,14 @@ _raw_stream, _raw_device = getattr(torch._C, "_cuda_getCurrentRawStream", None),
 _E4M3, _BF16, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.int32
 
 
+def _no_gradient(what: str, name: str, t: torch.Tensor) -> None:
+    """What would need a gradient, or carries a tangent of forward-mode differentiation, is refused: there is no formula for either."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: {name} requires a gradient, and there is none: call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what}: {name} carries a tangent, and there is none of the result")
+
+
 def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written: bool = False):
     """-> (the C structure, device index, rows, kv_heads, head_dim, positions that a row's table can hold)."""
     kind, shape, st, dev = k_pages.dtype, k_pages.shape, k_pages.stride(), k_pages.get_device()
@@ -167,6 +176,9 @@ def _paged_cache(what: str, k_pages, v_pages, table, k_scales, v_scales, written
         raise ValueError(f"{what}: v_pages must have the type, shape, strides and device of k_pages")
     if (k_pages.requires_grad or v_pages.requires_grad) and torch.is_grad_enabled():
         raise ValueError(f"{what}: the pages require a gradient, and there is none: call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0 and kind is _BF16:
+        _no_gradient(what, "k_pages", k_pages)
+        _no_gradient(what, "v_pages", v_pages)
     n_pages, kv_heads, page, hd = shape
     sp, sh, ss, last = st
     if last != 1:
@@ -204,8 +216,8 @@ def _paged_rows(what: str, name: str, t: torch.Tensor, shape, dev: int, out: boo
     if t.dtype is not _BF16 or t.shape != shape or t.get_device() != dev or st[2] != 1:
         raise ValueError(f"{what}: {name}: expected bfloat16 {tuple(shape)} on cuda:{dev} with contiguous last dimension, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: {name} requires a gradient, and there is none: call it under torch.no_grad()")
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _no_gradient(what, name, t)
     s0, s1, _ = st
     if shape[0] <= 1:
         s0 = 0
@@ -224,6 +236,16 @@ def _paged_ints(what: str, name: str, t: Optional[torch.Tensor], n: int, dev: in
     if t.dtype is not _I32 or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{what}: {name}: expected contiguous int32 [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _paged_tables(what: str, cos: torch.Tensor, sin: torch.Tensor, hd: int, dev: int):
+    st, shape = cos.stride(), cos.shape
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype is not _BF16 or t.shape != shape or len(st) != 2 or shape[1] != hd or t.get_device() != dev or t.stride() != st or st[1] != 1:
+            raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {hd}] on cuda:{dev} with contiguous rows, of the same strides")
+        if t.requires_grad or _forward_ad._current_level >= 0:
+            _no_gradient(what, name, t)
+    return cos.data_ptr(), sin.data_ptr(), shape[0], st[0] if shape[0] > 1 else hd
 
 
 def _launch_on(dev: int, call, what: str, *args) -> None:
@@ -261,11 +283,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     off_p, start_p = _paged_ints(what, "offsets", offsets, rows + 1, dev), _paged_ints(what, "start", start, rows, dev)
     rope, heads, qr, qo, ko = (0, 0, 0, 0), 0, (0, 0, 0), (0, 0, 0), (0, 0, 0)
     if cos is not None and sin is not None:
-        cst, cshape = cos.stride(), cos.shape
-        for t in (cos, sin):
-            if t.dtype is not _BF16 or t.shape != cshape or len(cst) != 2 or cshape[1] != hd or t.get_device() != dev or t.stride() != cst or cst[1] != 1:
-                raise ValueError(f"{what}: expected bfloat16 rotary tables [positions, {hd}] on cuda:{dev} with contiguous rows, of the same strides")
-        rope = (cos.data_ptr(), sin.data_ptr(), cshape[0], cst[0] if cshape[0] > 1 else hd)
+        rope = _paged_tables(what, cos, sin, hd, dev)
     elif cos is not None or sin is not None or q is not None:
         raise ValueError(f"{what}: cos and sin come together, and q needs them")
     if q is not None:

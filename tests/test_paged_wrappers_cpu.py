@@ -3,6 +3,10 @@ import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
 ROOT = Path(__file__).resolve().parent.parent
 
 
@@ -23,3 +27,26 @@ except ValueError as e:
 """
     got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.strip().endswith("refused"), got.stderr
+
+
+def test_gradients_and_tangents_are_refused():
+    """Of rows and of the rotary tables (through the checks themselves: on the CPU a call ends at its pages)."""
+    from merv_amd import ops
+    x = torch.ones(3, 2, 64, dtype=torch.bfloat16)
+    c = torch.ones(8, 64, dtype=torch.bfloat16)
+    wants, c_wants = x.clone().requires_grad_(), c.clone().requires_grad_()
+    rows = lambda t: ops._paged_rows("call", "k", t, (3, 2, 64), -1)  # noqa: E731
+    assert rows(x) == (x.data_ptr(), 128, 64)
+    assert ops._paged_tables("call", c, c, 64, -1) == (c.data_ptr(), c.data_ptr(), 8, 64)
+    for bad in (lambda: rows(wants), lambda: ops._paged_tables("call", c_wants, c, 64, -1), lambda: ops._paged_tables("call", c, c_wants, 64, -1)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            bad()
+        with torch.no_grad():
+            bad()
+    with fwd.dual_level():
+        rows(x)
+        ops._paged_tables("call", c, c, 64, -1)
+        dual, c_dual = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(c, torch.ones_like(c))
+        for bad in (lambda: rows(dual), lambda: ops._paged_tables("call", c_dual, c, 64, -1), lambda: ops._paged_tables("call", c, c_dual, 64, -1)):
+            with pytest.raises(ValueError, match="tangent"):
+                bad()
