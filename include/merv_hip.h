@@ -480,7 +480,7 @@ typedef struct merv_paged_cache {
  * offsets[b] <= t < offsets[b + 1] (device int32 [rows + 1], not decreasing), at position start[b] + t - offsets[b]; offsets = NULL: one token
  * a row, T = rows. A row with start[b] < 0 and tokens at or behind offsets[rows] are left alone in every output. k, v [T, kv_heads, hd], q, q_out
  * [T, heads, hd], k_out [T, kv_heads, hd] bf16 with token and head strides in elements; q = NULL (heads = 0) and k_out = NULL leave these out; q_out may be q
- * and k_out may be k. cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
+ * and k_out may be k, of the same strides; they share no memory with any other operand (two that begin at the same address are refused). cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
  * rounded to bf16 once. e4m3: a row's scale is the smallest power of two under which no finite element of the (bf16) row is over 448, 2^-126 at least;
  * the codes are rounded to nearest even; NaN and infinities become NaN. A position without a page in the table is not stored; with rotation, one
  * outside the tables or without a page is NaN in q_out and k_out. Two tokens of one call must not meet in one slot of one page. */
@@ -490,13 +490,14 @@ int merv_paged_cache_write(const merv_paged_cache *cache, const void *k, int64_t
                            int64_t k_out_stride, int64_t k_out_head_stride, const int32_t *offsets, const int32_t *start, int32_t T, int32_t heads,
                            void *stream);
 /* Cached keys and values back as bf16: k_out, v_out [T, kv_heads, hd]; token t is row b's (offsets as above, required) at position
- * (start ? start[b] : 0) + t - offsets[b]. A position without a page reads as NaN; rows with start[b] < 0 and tokens behind the last row are left alone. */
+ * (start ? start[b] : 0) + t - offsets[b]. A position without a page reads as NaN; rows with start[b] < 0 and tokens behind the last row are left alone.
+ * k_out and v_out share no memory with each other or the cache. */
 int merv_paged_cache_read(const merv_paged_cache *cache, void *k_out, int64_t k_out_stride, int64_t k_out_head_stride, void *v_out, int64_t v_out_stride,
                           int64_t v_out_head_stride, const int32_t *offsets, const int32_t *start, int32_t T, void *stream);
 /* out[b, h] = sum_j softmax_j(scale * q[b, h] . k[b, j]) v[b, j] over positions max(0, len - window) .. len - 1 of row b, len = lens[b] (device int32;
  * window <= 0: all); kv head = h / (heads / kv_heads). lse (may be NULL) [rows, heads] fp32 = ln sum_j exp(scale * q . k). len <= 0: out = 0 and lse = -inf. A
  * length over the table's capacity or a bad page among those the row reads: that row's out and lse are NaN. Keys and values behind a row's length,
- * in its last page or before its window, may hold anything, NaN among it. q, out [rows, heads, hd] bf16 by strides; workspace:
+ * in its last page or before its window, may hold anything, NaN among it. q, out [rows, heads, hd] bf16 by strides (out may be q, of the same strides); workspace:
  * merv_paged_decode_attention_workspace_bytes(...) bytes, 16-byte aligned, of any contents, not shared by calls that may run at the same time. */
 size_t merv_paged_decode_attention_workspace_bytes(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int64_t capacity);
 int merv_paged_decode_attention(const merv_paged_cache *cache, const void *q, int64_t q_stride, int64_t q_head_stride, void *out, int64_t out_stride,

@@ -1192,6 +1192,11 @@ extern "C" int merv_paged_cache_write(const merv_paged_cache* cache, const void*
     MERV_CHECK(paged_rows_ok(k, k_stride, k_head_stride) && paged_rows_ok(v, v_stride, v_head_stride) && paged_rows_ok(q, q_stride, q_head_stride) &&
                    paged_rows_ok(q_out, q_out_stride, q_out_head_stride) && paged_rows_ok(k_out, k_out_stride, k_out_head_stride),
                "merv_paged_cache_write: rows must be 16-byte aligned with strides that are multiples of 8");
+    // a workgroup writes rotated rows while others still read theirs: in place is a row over itself, nothing else
+    MERV_CHECK((!q_out || (q_out != k && q_out != v && q_out != k_out)) && (!k_out || (k_out != v && k_out != q)) &&
+                   (q_out != q || (q_out_stride == q_stride && q_out_head_stride == q_head_stride)) &&
+                   (k_out != k || (k_out_stride == k_stride && k_out_head_stride == k_head_stride)),
+               "merv_paged_cache_write: q_out and k_out must not share memory with another operand (q_out may be q and k_out may be k, of the same strides)");
     a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.q = (const bf16_t*)q;
     a.cos = (const bf16_t*)cos_t; a.sin = (const bf16_t*)sin_t;
     a.q_out = (bf16_t*)q_out; a.k_out = (bf16_t*)k_out;
@@ -1216,6 +1221,7 @@ extern "C" int merv_paged_cache_read(const merv_paged_cache* cache, void* k_out,
     MERV_CHECK(k_out && v_out && offsets, "merv_paged_cache_read: null argument");
     MERV_CHECK(paged_rows_ok(k_out, k_out_stride, k_out_head_stride) && paged_rows_ok(v_out, v_out_stride, v_out_head_stride),
                "merv_paged_cache_read: rows must be 16-byte aligned with strides that are multiples of 8");
+    MERV_CHECK(k_out != v_out, "merv_paged_cache_read: k_out and v_out must not share memory");
     a.k_out = (bf16_t*)k_out; a.v_out = (bf16_t*)v_out;
     a.offsets = offsets; a.start = start;
     a.ko_st = k_out_stride; a.ko_sh = k_out_head_stride; a.vo_st = v_out_stride; a.vo_sh = v_out_head_stride;
@@ -1245,6 +1251,8 @@ extern "C" int merv_paged_decode_attention(const merv_paged_cache* cache, const 
     MERV_CHECK(q && out && lens, "merv_paged_decode_attention: null argument");
     MERV_CHECK(paged_rows_ok(q, q_stride, q_head_stride) && paged_rows_ok(out, out_stride, out_head_stride),
                "merv_paged_decode_attention: rows must be 16-byte aligned with strides that are multiples of 8");
+    MERV_CHECK(out != q || (out_stride == q_stride && out_head_stride == q_head_stride),
+               "merv_paged_decode_attention: out must not share memory with q (it may be q, of the same strides)");
     const size_t need = paged_attention_workspace_bytes(cache->rows, heads, cache->kv_heads, cache->head_dim, (long)capacity);
     MERV_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "merv_paged_decode_attention: workspace too small (merv_paged_decode_attention_workspace_bytes) or not 16-byte aligned");

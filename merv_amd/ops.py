@@ -266,7 +266,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     """New tokens k, v [T, kv_heads, head_dim] bf16 into the pages, in one launch with the rotary embedding of k and of q [T, heads, head_dim] where
     cos, sin [positions, head_dim] bf16 are given. Token t is row b's where offsets[b] <= t < offsets[b + 1] (int32 [rows + 1]; None: one token a
     row, t = b), at position start[b] + t - offsets[b]; rows with start[b] < 0 and tokens behind offsets[rows] are left alone, in every output. Returns
-    the rotated queries (q_out, or a new tensor; q_out=q rotates in place), None without q; k_out takes the rotated keys as well. float8_e4m3fn pages:
+    the rotated queries (q_out, or a new tensor; q_out=q rotates in place), None without q; k_out takes the rotated keys as well (k_out=k: in place). Outputs share
+    no memory with other operands. float8_e4m3fn pages:
     quantised with one power-of-two scale for each token and head (k_scales, v_scales); what is not finite becomes NaN. Two tokens of a call must not lie in
     the same place of a page (rows may share pages that are only read)."""
     what = "paged_cache_write"

@@ -50,3 +50,25 @@ def test_gradients_and_tangents_are_refused():
         for bad in (lambda: rows(dual), lambda: ops._paged_tables("call", c_dual, c, 64, -1), lambda: ops._paged_tables("call", c, c_dual, 64, -1)):
             with pytest.raises(ValueError, match="tangent"):
                 bad()
+
+
+def test_outputs_that_are_other_operands_are_refused():
+    """A workgroup would write over rows that another one still reads (C entries, host checks alone)."""
+    from merv_amd import _lib
+    from test_paged_cpu import _cache
+    lib, c = _lib.load(), _cache()
+
+    def write(**kw):
+        a = dict(k=1 << 20, ks=128, kh=64, v=2 << 20, vs=128, vh=64, q=3 << 20, qs=128, qh=64, cos=64, sin=64, rl=10, rs=64, qo=4 << 20, qos=128, qoh=64, ko=5 << 20, kos=128,
+                 koh=64, off=64, start=64, T=5, H=2, st=0)
+        a.update(kw)
+        return lib.merv_paged_cache_write(c, *a.values())
+
+    for kw in (dict(qo=1 << 20), dict(qo=2 << 20), dict(qo=5 << 20), dict(ko=2 << 20), dict(ko=3 << 20), dict(ko=1 << 20, kos=256), dict(qo=3 << 20, qoh=128),
+               dict(v=1 << 20, ko=1 << 20)):
+        with pytest.raises(ValueError, match="must not share memory"):
+            _lib.check(write(**kw), "write")
+    with pytest.raises(ValueError, match="must not share memory"):
+        _lib.check(lib.merv_paged_cache_read(c, 64, 128, 64, 64, 128, 64, 64, 0, 3, 0), "read")
+    with pytest.raises(ValueError, match="must not share memory"):
+        _lib.check(lib.merv_paged_decode_attention(c, 64, 256, 64, 64, 512, 64, 0, 64, 4, 0, 1.0, 4096, 1 << 30, 0), "attention")
