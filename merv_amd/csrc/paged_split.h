@@ -61,4 +61,29 @@ MERV_HD bool paged_whole(int total, int most, int all, int grid) {
 // its sum in 2w.
 MERV_HD int paged_slot(int w, bool first_segment) { return 2 * w + (first_segment ? 0 : 1); }
 
+// What a call launches, from sizes alone (the rows' lengths are on the device). Where a row cannot be long, one workgroup for each pair takes it whole and
+// there is no join: up to 9 units, or 16 where there are pairs enough (the longest possible row then costs 18 us). Of eight waves where every pair has
+// a CU to itself and more than one round of four waves to do.
+// Measured, 16 bits, 128 dims, this and the split one: 9 units, 1 x 8 pairs 9.9 and 9.8 us, 1 x 32 10.8 and 12.2, 33 x 4 12.8 and 17.6; 16 units, 1 x 8 14.4 and 10.5 us,
+// 1 x 32 16.1 and 14.5, 8 x 8 16.1 and 16.5 (8 bits 16.0 and 13.9), 33 x 4 19.8 and 24.0. Eight and four waves: 4 units, 1 x 8 pairs 7.6 and 7.2 us; 9 units 9.9 and 11.5; 64 x 8 pairs of
+// 9 units 36.7 and 35.9.
+inline bool paged_direct(long units, long pairs) { return units <= 9 || (units <= 16 && pairs >= 128); }
+inline int paged_direct_waves(long units, long pairs) { return units > 4 && pairs <= 256 ? 8 : 4; }
+
+struct PagedPlan {
+    int head_blocks, workers, grid, waves;
+    bool direct;
+};
+inline PagedPlan paged_plan(int rows, int H, int kv_heads, long capacity) {
+    PagedPlan pl;
+    pl.head_blocks = (H / kv_heads + PAGED_HEAD_BLOCK - 1) / PAGED_HEAD_BLOCK;
+    const long units = (capacity + PAGED_UNIT - 1) / PAGED_UNIT;
+    const long pairs = (long)rows * kv_heads * pl.head_blocks, most = units * pairs;
+    pl.workers = (int)(most < PAGED_MAX_WORKERS ? most : PAGED_MAX_WORKERS);
+    pl.direct = paged_direct(units, pairs);
+    pl.waves = pl.direct ? paged_direct_waves(units, pairs) : 4;
+    pl.grid = (int)(pl.direct || (pairs > pl.workers && pairs <= PAGED_MOST_WHOLE) ? pairs : pl.workers);
+    return pl;
+}
+
 }  // namespace merv
