@@ -163,8 +163,12 @@ class LlamaBackbone:
             raise ValueError(f"unknown kv_cache `{kv_cache}` (static, paged or paged-e4m3)")
         if kv_cache == "static" and not torch.is_tensor(inputs_embeds):
             raise ValueError("prompts of several lengths need kv_cache='paged' or 'paged-e4m3'")
+        if len(inputs_embeds) == 0:
+            raise ValueError("generate_from_embeds: one prompt at least is needed")
         rows, dev = len(inputs_embeds), inputs_embeds[0].device
         if isinstance(prompt_ids, (list, tuple)):  # of several lengths: padded with a row's own first id (the penalty counts an id once)
+            if len(prompt_ids) != rows or not all(p.numel() for p in prompt_ids):
+                raise ValueError(f"generate_from_embeds: prompt_ids: expected one id at least for each of {rows} rows, got {[p.numel() for p in prompt_ids]}")
             most = max(p.numel() for p in prompt_ids)
             prompt_ids = torch.stack([torch.cat([p.reshape(-1), p.reshape(-1)[:1].expand(most - p.numel())]) for p in prompt_ids])
         top_p = 1.0 if top_p is None else float(top_p)

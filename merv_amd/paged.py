@@ -271,6 +271,8 @@ class PagedDecoder(StaticDecoder):
 
     def decode(self, token: torch.Tensor, use_graph: bool = True) -> torch.Tensor:
         """token [batch]: each row's token at its position -> logits behind it [batch, vocab] (fp32)."""
+        if token.shape != (self.B,):
+            raise ValueError(f"decode: expected {self.B} tokens, one a row, got {tuple(token.shape)}")
         if not all(self.held) or any(s >= r for s, r in zip(self.held, self.room)):
             raise ValueError(f"decode: rows hold {self.held} positions, with room for {self.room}")
         with torch.cuda.device(self.dev):  # a capture is of the current device's stream

@@ -126,3 +126,21 @@ def test_a_ragged_batch_takes_the_pages_it_needs(dev, kv):
     small = PagedDecoder(bb.llm, 768, 8, n_pages=18)
     with pytest.raises(ValueError, match="pages needed"):
         small.prefill(emb, room=7)
+
+
+def test_what_does_not_fit_the_rows_is_refused(dev):
+    from merv_amd.paged import PagedDecoder
+    bb = backbone(dev)
+    emb = prompts([9, 4], 256, dev)
+    dec = PagedDecoder(bb.llm, 64, 2)
+    dec.prefill(emb)
+    for bad in ([5], [5, 6, 7], [[5], [6]]):
+        with pytest.raises(ValueError, match="one a row"):
+            dec.decode(torch.tensor(bad, device=dev))
+    assert dec.held == [9, 4]
+    with pytest.raises(ValueError, match="one prompt at least"):
+        bb.generate_from_embeds([], max_new_tokens=2, kv_cache="paged")
+    ids = torch.tensor([7, 8], device=dev)
+    for bad in ([ids], [ids, ids[:0]], [ids, ids, ids]):
+        with pytest.raises(ValueError, match="prompt_ids"):
+            bb.generate_from_embeds(emb, max_new_tokens=2, kv_cache="paged", repetition_penalty=2.0, prompt_ids=bad)
