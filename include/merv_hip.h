@@ -455,7 +455,7 @@ int merv_map_pool_attention(const void *kv, const float *q, void *out, int32_t n
 /*
  * A paged key / value cache for batches of rows (sequences) of unlike length, and the attention of one new token for each row over it. The
  * reference decodes through HF's DynamicCache, one clip a call (merv/models/vidlms/merv.py:818-825); these carry the decoding step of several clips
- * or questions at once (merv_amd/llm.py, PagedDecoder). They came after ABI version 4's other entries and change none of them.
+ * or questions at once (merv_amd/paged.py, PagedDecoder). They came after ABI version 4's other entries and change none of them.
  *
  *  Pages: k_pages / v_pages hold element (page, kv head, slot, d) at page * stride_page + head * stride_head + slot * stride_token + d (the same strides
  *  for both), bf16 or OCP e4m3. With e4m3, scale byte (page, head, slot) is at page * scale_stride_page + head * scale_stride_head + slot and a number
@@ -482,7 +482,7 @@ typedef struct merv_paged_cache {
  * [T, heads, hd], k_out [T, kv_heads, hd] bf16 with token and head strides in elements; q = NULL (heads = 0) and k_out = NULL leave these out; q_out may be q
  * and k_out may be k, of the same strides; they share no memory with any other operand (two that begin at the same address are refused). cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
  * rounded to bf16 once. e4m3: a row's scale is the smallest power of two under which no finite element of the (bf16) row is over 448, 2^-126 at least;
- * the codes are rounded to nearest even; NaN and infinities become NaN. A position without a page in the table is not stored; with rotation, one
+ * the codes are rounded to nearest even (248 x 2^120 and more to 2^128, which reads back as infinity); NaN and infinities become NaN. A position without a page in the table is not stored; with rotation, one
  * outside the tables or without a page is NaN in q_out and k_out. Two tokens of one call must not meet in one slot of one page. */
 int merv_paged_cache_write(const merv_paged_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v, int64_t v_stride,
                            int64_t v_head_stride, const void *q, int64_t q_stride, int64_t q_head_stride, const void *cos_t, const void *sin_t,

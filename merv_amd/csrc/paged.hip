@@ -187,8 +187,9 @@ __global__ __launch_bounds__(256) void paged_write_kernel(PagedWriteArgs p) {
 
 // ---- read ----
 // The same line of vectors, READ_EACH for each group of lanes: all places first, then all loads, then all stores. A lane moves 16 bytes of the cache.
-// Bound by HBM: 32 rows of up to 4000 positions (2 kv heads, bf16, 154 MB moved) 27.0 us, 5.7 TB/s with two, 29.0 with one, 28.5 with four; 41.4 without
-// non-temporal stores. 1049 positions (8 kv heads, e4m3): 4.0 us with one, 4.8 with two.
+// Bound by memory: 32 rows of up to 4000 positions (2 kv heads, bf16, 154 MB moved) 27.0 us, 5.7 TB/s with two, 29.0 with one, 28.5 with four; 41.4 without
+// non-temporal stores (repeated calls: these pages, 77 MB, stay in the 256 MB Infinity Cache). e4m3 of the same rows 23.9 us, 4.9 TB/s. Pages beyond that cache:
+// 32 x 4000, 8 kv heads, bf16 142 us, 4.3 TB/s; 32 x 8000, e4m3 222 us, 4.3. 1049 positions (8 kv heads, e4m3): 3.9 us with one, 4.8 with two.
 template <int HD, bool E4M3, int READ_EACH>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
     constexpr int LPV = E4M3 ? HD / 16 : HD / 8, VPB = 256 / LPV, EPL = HD / LPV;
@@ -248,7 +249,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
 // (v_perm_b32), row r of product dt being dim r * HD/16 + dt. K's operand wants a key in a lane: loaded so, a wave's 64 16-byte pieces lie in 16 lines of memory
 // (62 GB/s a CU); loaded in whole lines and turned in the wave's own corner of LDS, 80 (16 bits; one row of 4096 positions, unsplit, 38.6 and 30.2 us).
 // Scores, maximum, sum and output are fp32, and so are the weights: the 24 bits of a p are three bf16 numbers of 8 each (split_weight), whose products with
-// bf16 values are exact in fp32. Two of them (2^-17 off) turned 0.3 - 0.6 % of the outputs to the other side of their rounding.
+// bf16 values are exact in fp32. Two of them (2^-17 off) turned 0.3 - 0.6 % of the outputs to the other side of their rounding; the
+// third costs 0.6 of 22 us where a call is bound by instructions (33 rows of up to 3001, 8 bits), elsewhere nothing.
 // The running maximum moves only when a weight would exceed 2^RAISE: the rescaling of the 32 output registers is then rare. A row's weights may so add up to
 // 2^RAISE times its positions; they and their sum are used 2^-shift times that, `shift` chosen from the longest possible row, so that a sum
 // of weighted values never exceeds the largest value: the result is finite where the formula's is. (Weights and values whose product is under
@@ -634,8 +636,8 @@ MERV_DEVICE void end_worker(const PagedAttnArgs& p, PagedOpen open, const PagedS
 //
 // Bound by HBM where the call is large, by its chain of round trips (length, pages, keys and values, sums) where it is small. Measured, 128 dims:
 //   96 rows of 2458 .. 8192 positions, 32 / 8 heads, 16 bits: 352 us, 5.87 TB/s of keys and values (a copy of 1 GiB on this card: 5.05)
-//   1 row of 131072, 32 / 8 heads, 8 bits: 58 us, 4.7 TB/s, 6 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 21.7 us, 2.8 TB/s
-//   1 row of 77, 16 / 2 heads: 4.5 us;  1 row of 1049, 32 / 32, 16 bits: 11.2 us
+//   1 row of 131072, 32 / 8 heads, 8 bits: 58.6 us, 4.6 TB/s, 6 of them the join;  33 rows of up to 3001, 28 / 4, 8 bits: 22.4 us, 2.7 TB/s
+//   1 row of 77, 16 / 2 heads: 4.5 us;  1 row of 1049, 32 / 32, 16 bits: 11.5 us in a table of 1088 positions (one launch), 12.0 in one of 1280 (shared out)
 // 512 workers: with 1024 the large call takes 363 us and 33 x 3001 takes a fifth more (twice the segments); with 256 half the loads are on their way.
 // Two workgroups a CU: 8 waves x 2 tiles of 16 KB (16 bits) outstanding cover the latency; registers, not LDS, set the limit (three for 8 bits: 33
 // registers spill, 33 x 3001 takes 25.9 us, 131072 75.5).

@@ -64,9 +64,14 @@ MERV_HD int paged_slot(int w, bool first_segment) { return 2 * w + (first_segmen
 // What a call launches, from sizes alone (the rows' lengths are on the device). Where a row cannot be long, one workgroup for each pair takes it whole and
 // there is no join: up to 9 units, or 16 where there are pairs enough (the longest possible row then costs 18 us). Of eight waves where every pair has
 // a CU to itself and more than one round of four waves to do.
-// Measured, 16 bits, 128 dims, this and the split one: 9 units, 1 x 8 pairs 9.9 and 9.8 us, 1 x 32 10.8 and 12.2, 33 x 4 12.8 and 17.6; 16 units, 1 x 8 14.4 and 10.5 us,
-// 1 x 32 16.1 and 14.5, 8 x 8 16.1 and 16.5 (8 bits 16.0 and 13.9), 33 x 4 19.8 and 24.0. Eight and four waves: 4 units, 1 x 8 pairs 7.6 and 7.2 us; 9 units 9.9 and 11.5; 64 x 8 pairs of
-// 9 units 36.7 and 35.9.
+// Measured, 128 dims, this and the split one in us (16 bits; 8 bits where they differ by more):
+//   9 units   1 x 8 pairs 10.5,  9.8; 1 x 32 11.6, 12.5 (11.1, 11.1); 8 x 8 11.8, 14.0; 33 x 4 12.8, 17.6
+//   10 units  1 x 8 11.5,  9.8; 1 x 32 12.6, 13.1 (12.1, 11.1); 8 x 8 12.6, 13.2 (12.1, 11.5); a row of 1049 in a table of 1280, 1 x 32: 11.1, 12.0 (11.0, 11.1)
+//   12 units  1 x 8 12.7,  9.9; 1 x 32 14.0, 13.4 (13.6, 11.2); 8 x 8 13.9, 14.7 (13.8, 12.1)
+//   14 units  1 x 8 14.2, 10.5; 1 x 32 15.2, 14.3 (15.2, 12.1); 8 x 8 15.4, 16.0 (15.5, 13.3)
+//   16 units  1 x 8 15.4, 10.5; 1 x 32 16.5, 14.6 (16.6, 12.7); 8 x 8 16.4, 16.8 (16.8, 13.7); 33 x 4 19.8, 24.0
+// Between 9 and 16 units neither form is the better one for all pairs and both types; the most that the rule gives away there is 2.5 us (2 x 32 pairs, 16 bits,
+// 10 units: 12.8, 15.3). Eight and four waves: 4 units, 1 x 8 pairs 7.6 and 7.2 us; 9 units 9.9 and 11.5; 64 x 8 pairs of 9 units 36.7 and 35.9.
 inline bool paged_direct(long units, long pairs) { return units <= 9 || (units <= 16 && pairs >= 128); }
 inline int paged_direct_waves(long units, long pairs) { return units > 4 && pairs <= 256 ? 8 : 4; }
 

@@ -157,8 +157,10 @@ class LlamaBackbone:
         as in HF's GenerationConfig.
 
         kv_cache "paged" / "paged-e4m3": a paged cache in bf16 / 8 bits (merv_amd.paged.PagedDecoder). `inputs_embeds` may then be a list of [S_b, D], prompts
-        of lengths of their own (and `prompt_ids` a list of 1-D tensors); all rows are decoded together. Up to the 8-bit rounding the tokens are those that
-        each prompt alone would get, behind a row's end of sequence they mean nothing."""
+        of lengths of their own (and `prompt_ids` a list of 1-D tensors); all rows are decoded together, on the pages that they need. Each row's tokens are
+        those of its prompt alone but for the cache's 8-bit rounding and the order of the sums, which changes with the batch: near ties may fall the other way.
+        Behind a row's end of sequence they mean nothing. For ONE row the static cache's HipDecoder is faster (0.70 against 1.34 ms a step of 8 layers of
+        Llama-2-7B at 1049 positions)."""
         if kv_cache not in ("static", "paged", "paged-e4m3"):
             raise ValueError(f"unknown kv_cache `{kv_cache}` (static, paged or paged-e4m3)")
         if kv_cache == "static" and not torch.is_tensor(inputs_embeds):

@@ -144,7 +144,7 @@ def gemm_mxfp8(aq, a_sc, wq, w_sc, bias=None, act="none", lscale=None, res=None,
     return out
 
 
-# ---- paged key / value cache (PagedDecoder, llm.py): rows of unlike length on one pool of pages ----
+# ---- paged key / value cache (PagedDecoder, paged.py): rows of unlike length on one pool of pages ----
 # Pages are [n_pages, kv_heads, page_size, head_dim], bf16 or torch.float8_e4m3fn (then with uint8 scales [n_pages, kv_heads, page_size], a number
 # standing for code * 2^(byte - 127)); table [rows, width] int32 names the page of positions i * page_size .. of a row. Any strides, last
 # dimension contiguous. Row lengths, offsets and page numbers stay on the device (a captured step replays with new ones); the kernels check
@@ -309,7 +309,8 @@ def paged_cache_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.
                      k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
     """Cached keys and values, back as bf16 [total, kv_heads, head_dim] each, rows one behind the other: output t is row b's position
     (start[b] or 0) + t - offsets[b] where offsets[b] <= t < offsets[b + 1]. Outputs behind offsets[rows], and those of rows with start[b] < 0, are
-    not written. A position without a page reads as NaN. Numbers are given back exactly as the cache holds them."""
+    not written. A position without a page reads as NaN. Numbers are given back exactly as the cache holds
+    them; e4m3 rows with numbers of 248 x 2^120 and more (bf16's eight largest) hold 2^128 there, which bf16 has no finite number for: infinity."""
     what = "paged_cache_read"
     cache, dev, rows, kv_heads, hd, _ = _paged_cache(what, k_pages, v_pages, table, k_scales, v_scales)
     total = int(total)

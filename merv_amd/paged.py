@@ -202,9 +202,7 @@ class PagedDecoder(StaticDecoder):
             for n in ends:
                 all_off.append(all_off[-1] + n)
             all_off_d = i32(all_off)
-        x = torch.cat([e.to(device=self.dev, dtype=self.dt) for e in embeds], 0).contiguous()
-        if len(embeds) == 1 and x.data_ptr() == embeds[0].data_ptr():
-            x = x.clone()  # the residual stream is updated in place
+        x = torch.cat([e.to(device=self.dev, dtype=self.dt) for e in embeds], 0)  # (a copy, also of one row: the residual stream is updated in place)
         st = torch.cuda.current_stream(self.dev).cuda_stream
 
         def attend(li, q, k, v):
@@ -270,7 +268,8 @@ class PagedDecoder(StaticDecoder):
             return self._logits(self._layers(x, attend))
 
     def decode(self, token: torch.Tensor, use_graph: bool = True) -> torch.Tensor:
-        """token [batch]: each row's token at its position -> logits behind it [batch, vocab] (fp32)."""
+        """token [batch]: each row's token at its position -> logits behind it [batch, vocab] (fp32; a captured step's own tensor, which the next step
+        writes over)."""
         if token.shape != (self.B,):
             raise ValueError(f"decode: expected {self.B} tokens, one a row, got {tuple(token.shape)}")
         if not all(self.held) or any(s >= r for s, r in zip(self.held, self.room)):

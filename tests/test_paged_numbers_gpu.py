@@ -109,3 +109,21 @@ def test_long_stretches_of_one_row(dev, fmt, hd, window):
     good[rows] = False
     w = which[good]
     assert ((out[good] - want[w]).abs() <= tol[w]).all() and ((lse[good] - want_l[w]).abs() <= tol_l[w]).all()
+
+
+def test_the_largest_numbers_round_to_infinity_in_e4m3(dev):
+    """From 248 x 2^120 on the nearest e4m3 number is 256 x 2^120 = 2^128: infinite as bf16, in what is read and what is attended to. Below: finite."""
+    from merv_amd import ops
+    hd, step = 64, 2.0**120
+    x = torch.tensor([255.0, 248.0, 247.0, -255.0, -247.0], dtype=P.F64)[:, None].expand(-1, hd) * step
+    pool = P.Pool([5] * 5, 1, hd, 16, "e4m3", dev)
+    k = torch.zeros(5, 1, hd, dtype=torch.bfloat16, device=dev)
+    v = x.to(torch.bfloat16)[:, None].to(dev)
+    assert torch.equal(v[:, 0].cpu().to(P.F64), x)
+    table, one = pool.table.to(dev), i32([1] * 5, dev)
+    ops.paged_cache_write(k, v, pool.k, pool.v, table, i32([0] * 5, dev), **pool.scales())
+    want = torch.tensor([math.inf, math.inf, 240 * step, -math.inf, -240 * step], dtype=P.F64)[:, None].expand(-1, hd)
+    _, back = ops.paged_cache_read(pool.k, pool.v, table, None, i32([0, 1, 2, 3, 4, 5], dev), 5, **pool.scales())
+    assert torch.equal(back[:, 0].cpu().to(P.F64), want)
+    out = ops.paged_decode_attention(torch.ones(5, 1, hd, dtype=torch.bfloat16, device=dev), pool.k, pool.v, table, one, **pool.scales())
+    assert torch.equal(out[:, 0].cpu().to(P.F64), want)
