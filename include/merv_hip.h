@@ -480,9 +480,11 @@ typedef struct merv_paged_cache {
  * offsets[b] <= t < offsets[b + 1] (device int32 [rows + 1], not decreasing), at position start[b] + t - offsets[b]; offsets = NULL: one token
  * a row, T = rows. A row with start[b] < 0 and tokens at or behind offsets[rows] are left alone in every output. k, v [T, kv_heads, hd], q, q_out
  * [T, heads, hd], k_out [T, kv_heads, hd] bf16 with token and head strides in elements; q = NULL (heads = 0) and k_out = NULL leave these out; q_out may be q
- * and k_out may be k, of the same strides; they share no memory with any other operand (two that begin at the same address are refused). cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
+ * and k_out may be k, of the same strides; they share no memory with any other operand (two that begin at the same address are refused).
+ * cos, sin [rope_len, hd] bf16, row stride rope_stride; both NULL: no rotation (q must be NULL). rot = x cos + rotate_half(x) sin in fp32,
  * rounded to bf16 once. e4m3: a row's scale is the smallest power of two under which no finite element of the (bf16) row is over 448, 2^-126 at least;
- * the codes are rounded to nearest even (248 x 2^120 and more to 2^128, which reads back as infinity); NaN and infinities become NaN. A position without a page in the table is not stored; with rotation, one
+ * the codes are rounded to nearest even (248 x 2^120 and more to 2^128, which reads back as infinity); NaN and infinities become NaN.
+ * A position without a page in the table is not stored; with rotation, one
  * outside the tables or without a page is NaN in q_out and k_out. Two tokens of one call must not meet in one slot of one page. */
 int merv_paged_cache_write(const merv_paged_cache *cache, const void *k, int64_t k_stride, int64_t k_head_stride, const void *v, int64_t v_stride,
                            int64_t v_head_stride, const void *q, int64_t q_stride, int64_t q_head_stride, const void *cos_t, const void *sin_t,

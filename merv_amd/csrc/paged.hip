@@ -253,8 +253,8 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedReadArgs p) {
 // third costs 0.6 of 22 us where a call is bound by instructions (33 rows of up to 3001, 8 bits), elsewhere nothing.
 // The running maximum moves only when a weight would exceed 2^RAISE: the rescaling of the 32 output registers is then rare. A row's weights may so add up to
 // 2^RAISE times its positions; they and their sum are used 2^-shift times that, `shift` chosen from the longest possible row, so that a sum
-// of weighted values never exceeds the largest value: the result is finite where the formula's is. (Weights and values whose product is under
-// 2^(shift - 126), with a shift of 20 for 16384 positions, lose bits to fp32's smallest numbers.)
+// of weighted values never exceeds the largest value: the result is finite where the formula's is. (At the other end fp32's smallest numbers begin: weights, with e4m3
+// times their value's power of two, under 2^(shift - 102) lose bits, and are NaN with an infinite value; the shift is 20 for 16384 positions.)
 // e4m3 codes become bf16 exactly; a key's power of two multiplies its score, a value's its weight.
 constexpr int RAISE = 6;
 
@@ -337,7 +337,7 @@ struct PagedState {  // of a wave: lane l has head l % 16
 };
 
 // p >= 0 as the sum of three bf16 numbers (the upper halves of x), exactly: p cut off behind 8 bits, the rest cut off, the rest of that, which has 8 bits left.
-// POSITIVE, where values may be infinite: all three parts of a p > 0 are over zero, so that none turns an infinity round or makes it NaN. For that the number
+// POSITIVE, where values may be infinite: all three parts of a p >= 2^-102 are over zero, so that none turns an infinity round or makes it NaN. For that the number
 // before p is cut off instead of p: what is left is over zero and, where p itself had 8 bits only, a power of two.
 template <bool POSITIVE>
 MERV_DEVICE void split_weight(float p, uint32_t (&x)[3]) {

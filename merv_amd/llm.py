@@ -169,8 +169,8 @@ class LlamaBackbone:
             raise ValueError("generate_from_embeds: one prompt at least is needed")
         rows, dev = len(inputs_embeds), inputs_embeds[0].device
         if isinstance(prompt_ids, (list, tuple)):  # of several lengths: padded with a row's own first id (the penalty counts an id once)
-            if len(prompt_ids) != rows or not all(p.numel() for p in prompt_ids):
-                raise ValueError(f"generate_from_embeds: prompt_ids: expected one id at least for each of {rows} rows, got {[p.numel() for p in prompt_ids]}")
+            if len(prompt_ids) != rows or len({p.numel() > 0 for p in prompt_ids}) > 1:
+                raise ValueError(f"generate_from_embeds: prompt_ids: expected one id at least for each of {rows} rows, or none for all, got {[p.numel() for p in prompt_ids]}")
             most = max(p.numel() for p in prompt_ids)
             prompt_ids = torch.stack([torch.cat([p.reshape(-1), p.reshape(-1)[:1].expand(most - p.numel())]) for p in prompt_ids])
         top_p = 1.0 if top_p is None else float(top_p)

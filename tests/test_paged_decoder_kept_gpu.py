@@ -144,3 +144,5 @@ def test_what_does_not_fit_the_rows_is_refused(dev):
     for bad in ([ids], [ids, ids[:0]], [ids, ids, ids]):
         with pytest.raises(ValueError, match="prompt_ids"):
             bb.generate_from_embeds(emb, max_new_tokens=2, kv_cache="paged", repetition_penalty=2.0, prompt_ids=bad)
+    none = bb.generate_from_embeds(emb, max_new_tokens=4, kv_cache="paged", repetition_penalty=2.0, prompt_ids=[ids[:0], ids[:0]])
+    assert torch.equal(none, bb.generate_from_embeds(emb, max_new_tokens=4, kv_cache="paged", repetition_penalty=2.0))
